@@ -1,0 +1,145 @@
+// Shared by the position-wise layers (linear.hip, layernorm.hip, dropout.hip): the element types,
+// vector access at any element alignment, the activations and the dropout generator.
+#pragma once
+#include "gwn_internal.h"
+
+namespace elem {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+// 16 bytes of elements: one global_load_dwordx4 per lane
+template <typename T> struct Vec { static constexpr int N = 16 / (int)sizeof(T); };
+
+// n-element access aligned to the element only (rows of odd widths start anywhere): the packed
+// struct tells the compiler the alignment, and gfx950 loads and stores dwords at any byte address
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load(const T* p) {
+  return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const Pack<T, N>& v) {
+  *reinterpret_cast<Pack<T, N>*>(p) = v;
+}
+
+// ---- dropout ---------------------------------------------------------------------------------
+// Counter based: element i of a tensor is kept by the mask of (seed, salt) iff u24(i) >= thr, thr =
+// ceil(p 2^24).  The 64-bit key is two rounds of the SplitMix64 finaliser (Steele, Lea and Flood
+// 2014) over seed, salt and the high half of i; its low word starts the 32-bit mix of the low half
+// (the constants of gwn_mix32), its high word enters between that mix's two multiplies, so that two
+// keys' streams are not shifts of one another.  Two multiplies per element, no memory: the mask is
+// the same in every kernel that applies or differentiates it.
+struct Drop {
+  const unsigned long long* seed_ptr;
+  unsigned long long salt;
+  unsigned thr;  // 0: no dropout
+  float scale;   // 1 / (1 - p); 0 for p = 1
+};
+
+__host__ __device__ inline unsigned long long mix64(unsigned long long v) {
+  v = (v ^ (v >> 30)) * 0xBF58476D1CE4E5B9ull;
+  v = (v ^ (v >> 27)) * 0x94D049BB133111EBull;
+  return v ^ (v >> 31);
+}
+
+struct DropKey {
+  unsigned long long base;
+  unsigned hi, k0, k1;
+  __device__ __forceinline__ void rekey(unsigned h) {
+    const unsigned long long k = mix64(base + h);
+    hi = h;
+    k0 = (unsigned)k;
+    k1 = (unsigned)(k >> 32);
+  }
+  __device__ __forceinline__ void init(const Drop& d, unsigned long long i) {
+    base = mix64(*d.seed_ptr + 0x9E3779B97F4A7C15ull * (d.salt + 1));
+    // a wave's elements share the high half but where it steps: keyed once, on the scalar unit
+    rekey(__builtin_amdgcn_readfirstlane((unsigned)(i >> 32)));
+  }
+  __device__ __forceinline__ void seek(unsigned long long i) {
+    if ((unsigned)(i >> 32) != hi) rekey((unsigned)(i >> 32));
+  }
+  // of element i, the high half of which seek() has set
+  __device__ __forceinline__ bool keep(unsigned lo, unsigned thr) const {
+    unsigned h = lo * 0x9E3779B1u + k0;
+    h ^= h >> 16;
+    h *= 0x7FEB352Du;
+    h ^= h >> 15;
+    h += k1;
+    h *= 0x846CA68Bu;
+    h ^= h >> 16;
+    return (h >> 8) >= thr;
+  }
+};
+
+// ---- activations -----------------------------------------------------------------------------
+// FAST (16-bit results): exp and reciprocal by the hardware's instructions, erf by Abramowitz and
+// Stegun 7.1.26 (absolute error 1.5e-7, a hundredth of half a step of f16 at 1).
+template <bool FAST> __device__ __forceinline__ float exp_(float x) { return FAST ? __expf(x) : expf(x); }
+template <bool FAST> __device__ __forceinline__ float rcp_(float x) {
+  return FAST ? __builtin_amdgcn_rcpf(x) : 1.0f / x;
+}
+
+// the normal distribution's Phi(z); e = exp(-z^2 / 2)
+template <bool FAST> __device__ __forceinline__ float normal_cdf(float z, float e) {
+  if (!FAST) return 0.5f * erfcf(-0.70710678f * z);
+  const float t = rcp_<true>(1.0f + 0.3275911f * 0.70710678f * fabsf(z));
+  const float p =
+      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * p * e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
+template <bool FAST> __device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case GWN_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
+    case GWN_ACT_GELU: return z * normal_cdf<FAST>(z, FAST ? exp_<FAST>(-0.5f * z * z) : 0.0f);
+    case GWN_ACT_GELU_TANH: {
+      const float u = z * (1.5957691216f + 0.0713548163f * z * z);  // 2 sqrt(2/pi) (z + 0.044715 z^3)
+      return z * rcp_<FAST>(1.0f + exp_<FAST>(-u));
+    }
+    case GWN_ACT_SILU: return z * rcp_<FAST>(1.0f + exp_<FAST>(-z));
+    default: return z;
+  }
+}
+
+// the derivative; past |z| = 50 every one of them is 0 or 1 to the last bit, and the formulas'
+// products of an infinity and a zero are not formed
+template <bool FAST> __device__ __forceinline__ float act_slope(float z, int act) {
+  if (act == GWN_ACT_NONE) return 1.0f;
+  if (act == GWN_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (z > 50.0f) return 1.0f;
+  if (z < -50.0f) return 0.0f;
+  if (act == GWN_ACT_GELU) {
+    const float e = exp_<FAST>(-0.5f * z * z);
+    return normal_cdf<FAST>(z, e) + 0.3989422804f * z * e;
+  }
+  if (act == GWN_ACT_GELU_TANH) {
+    const float z2 = z * z, u = z * (1.5957691216f + 0.0713548163f * z2);
+    const float s = rcp_<FAST>(1.0f + exp_<FAST>(-u));
+    return s + z * s * (1.0f - s) * (1.5957691216f + 0.2140644488f * z2);
+  }
+  const float s = rcp_<FAST>(1.0f + exp_<FAST>(-z));
+  return s * (1.0f + z * (1.0f - s));
+}
+
+template <typename T> constexpr bool is16 = sizeof(T) == 2;
+
+inline int elem_bytes(int e) { return e == GWN_ELEM_F32 ? 4 : 2; }
+inline bool elem_ok(int e) { return e == GWN_ELEM_F32 || e == GWN_ELEM_F16 || e == GWN_ELEM_BF16; }
+
+// p in [0, 1] -> the kernel's threshold and scale
+inline Drop drop_of(const unsigned long long* seed_ptr, unsigned long long salt, double p) {
+  Drop d{seed_ptr, salt, 0u, 1.0f};
+  const double t = p * 16777216.0;
+  d.thr = (unsigned)t;
+  if ((double)d.thr < t) ++d.thr;
+  d.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+  return d;
+}
+
+}  // namespace elem

@@ -1022,6 +1022,8 @@ long gwn_abi_sizeof(const char* name) {
   if (!strcmp(name, "gwn_wgrad_problem")) return (long)sizeof(gwn_wgrad_problem);
   if (!strcmp(name, "gwn_gram_layer")) return (long)sizeof(gwn_gram_layer);
   if (!strcmp(name, "gwn_bn_fold")) return (long)sizeof(gwn_bn_fold);
+  if (!strcmp(name, "gwn_linear_args")) return (long)sizeof(gwn_linear_args);
+  if (!strcmp(name, "gwn_linear_bwd_args")) return (long)sizeof(gwn_linear_bwd_args);
   return -1;
 }
 

@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("GWN_LIB") or os.path.join(_HERE, "libgwn.so")
 
 c_int, c_long, c_float, c_void_p, c_u64 = (ctypes.c_int, ctypes.c_long, ctypes.c_float,
                                           ctypes.c_void_p, ctypes.c_ulonglong)
+c_double = ctypes.c_double
 
 
 class GemmDesc(ctypes.Structure):
@@ -166,11 +167,44 @@ class GcnBwdArgs(ctypes.Structure):
         ("tg4", c_void_p),
     ]
 
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("ldx", c_long),
+        ("w", c_void_p), ("ldw", c_long),
+        ("bias", c_void_p),
+        ("residual", c_void_p), ("ld_res", c_long),
+        ("y", c_void_p), ("ldy", c_long),
+        ("z", c_void_p), ("ldz", c_long),
+        ("M", c_int), ("N", c_int), ("K", c_int),
+        ("elem", c_int), ("act", c_int),
+        ("seed_ptr", c_void_p), ("salt", c_u64), ("drop_p", c_double),
+        ("workspace", c_void_p),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", c_void_p), ("ld_dy", c_long),
+        ("x", c_void_p), ("ldx", c_long),
+        ("w", c_void_p), ("ldw", c_long),
+        ("z", c_void_p), ("ldz", c_long),
+        ("dx", c_void_p), ("ld_dx", c_long),
+        ("dw", c_void_p), ("ld_dw", c_long),
+        ("dbias", c_void_p),
+        ("M", c_int), ("N", c_int), ("K", c_int),
+        ("elem", c_int), ("act", c_int),
+        ("seed_ptr", c_void_p), ("salt", c_u64), ("drop_p", c_double),
+        ("workspace", c_void_p),
+    ]
+
+
 # ctypes mirrors checked against the library's own sizeof (gwn_abi_sizeof) at load time
 _STRUCTS = {"gwn_gemm_desc": GemmDesc, "gwn_tcn_args": TcnArgs, "gwn_tcn_bwd_args": TcnBwdArgs,
             "gwn_gcn_args": GcnArgs, "gwn_gcn_bwd_args": GcnBwdArgs, "gwn_reduce_seg": ReduceSeg,
             "gwn_wgrad_problem": WgradProblem, "gwn_gram_layer": GramLayer,
-            "gwn_bn_fold": BnFold}
+            "gwn_bn_fold": BnFold, "gwn_linear_args": LinearArgs, "gwn_linear_bwd_args": LinearBwdArgs}
 
 
 # (name, restype, argtypes) of every exported entry point declared in include/gwn.h
@@ -294,6 +328,16 @@ _SIGS = [
     ("gwn_gather_rows", c_int, [c_void_p, c_long, c_void_p, c_int, c_void_p, c_void_p]),
     ("gwn_window_batch", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                  c_int, ctypes.c_double, ctypes.c_double, c_int, c_void_p, c_void_p, c_void_p]),
+    ("gwn_dropout", c_int, [c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p, c_u64, c_double, c_void_p]),
+    ("gwn_layernorm_fwd", c_int, [c_void_p, c_long, c_long, c_int, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p,
+                                  c_long, c_void_p, c_void_p, c_void_p]),
+    ("gwn_layernorm_bwd", c_int, [c_void_p, c_long, c_void_p, c_long, c_long, c_int, c_int, c_void_p, c_int, c_void_p,
+                                  c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("gwn_layernorm_bwd_workspace_floats", c_long, [c_long, c_int, c_int]),
+    ("gwn_linear_fwd", c_int, [ctypes.POINTER(LinearArgs), c_void_p]),
+    ("gwn_linear_fwd_workspace_floats", c_long, [c_int, c_int, c_int, c_int]),
+    ("gwn_linear_bwd", c_int, [ctypes.POINTER(LinearBwdArgs), c_void_p]),
+    ("gwn_linear_bwd_workspace_floats", c_long, [c_int, c_int, c_int, c_int]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]

@@ -46,7 +46,8 @@ void gwn_set_sync_check(int mode);
 const char* gwn_last_error(void);
 /* sizeof of the argument structs below, for bindings that mirror them (ctypes, cgo):
  * "gwn_gemm_desc", "gwn_tcn_args", "gwn_tcn_bwd_args", "gwn_gcn_args", "gwn_gcn_bwd_args",
- * "gwn_reduce_seg", "gwn_wgrad_problem", "gwn_gram_layer", "gwn_bn_fold";
+ * "gwn_reduce_seg", "gwn_wgrad_problem", "gwn_gram_layer", "gwn_bn_fold", "gwn_linear_args",
+ * "gwn_linear_bwd_args";
  * -1 for an unknown name */
 long gwn_abi_sizeof(const char* struct_name);
 
@@ -751,6 +752,88 @@ int gwn_gather_rows(const float* src, long row_floats, const long long* idx, int
 int gwn_window_batch(const double* series, const double* tod, const double* dow, int N,
                      const long long* t_last, int B, const int* xoff, int LX, const int* yoff, int LY,
                      double mean, double std, int scale_x, float* x, float* y, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Position-wise layers over channels-last rows: the product with its epilogue, layer norm, and
+ * dropout without a stored mask, with their backward passes, for f32, f16 and bf16 tensors.  They
+ * extend linear (model.py:24-30), the BatchNorm (model.py:152, 236) and the dropout (model.py:54)
+ * of the graph convolution; the reference has no counterpart.  Sums, statistics and gradients'
+ * partial sums are fp32 whatever the element type, every output is rounded once, and reductions
+ * have a fixed order.  Pointers are aligned to their element, no more; a leading dimension counts
+ * elements and is at least the row's length.  Outputs must not overlap inputs unless said.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum gwn_elem { GWN_ELEM_F32 = 0, GWN_ELEM_F16 = 1, GWN_ELEM_BF16 = 2 } gwn_elem;
+typedef enum gwn_act {
+  GWN_ACT_NONE = 0,
+  GWN_ACT_RELU = 1,
+  GWN_ACT_GELU = 2,      /* z Phi(z), Phi by erf */
+  GWN_ACT_GELU_TANH = 3, /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+  GWN_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+} gwn_act;
+
+/* y_i = residual_i + keep(i) x_i / (1 - drop_p) over `count` elements; residual NULL = none; y may
+ * be x or residual.  Element i is kept iff u24(i) >= ceil(drop_p 2^24): with
+ *   mix64(v): v = (v ^ v>>30) * 0xBF58476D1CE4E5B9; v = (v ^ v>>27) * 0x94D049BB133111EB; v ^ v>>31
+ *   k = mix64(mix64(*seed_ptr + 0x9E3779B97F4A7C15 (salt + 1)) + (i >> 32))
+ *   h = (unsigned)i * 0x9E3779B1 + low32(k);  h ^= h>>16;  h *= 0x7FEB352D;  h ^= h>>15;
+ *   h += high32(k);  h *= 0x846CA68B;  h ^= h>>16;  u24 = h >> 8.
+ * A dropped element is 0 whatever x holds there.  The backward is the same call on dy without a
+ * residual, with *seed_ptr as it was (dresidual = dy). */
+int gwn_dropout(const void* x, const void* residual, void* y, long count, int elem,
+                const unsigned long long* seed_ptr, unsigned long long salt, double drop_p, hipStream_t stream);
+
+/* Layer norm over the c values of each of `rows` rows:
+ *   mean = sum x / c, rstd = 1/sqrt(sum (x - mean)^2 / c + eps), y = (x - mean) rstd gamma + beta.
+ * gamma / beta [c] (NULL = 1 / 0) are of type `elem`, or f32 with params_f32 != 0.  mean / rstd
+ * [rows] f32 (both or neither NULL) are kept for the backward.  y may be x (same ld). */
+int gwn_layernorm_fwd(const void* x, long ldx, long rows, int c, int elem, const void* gamma, const void* beta,
+                      int params_f32, float eps, void* y, long ldy, float* mean, float* rstd, hipStream_t stream);
+/* its gradients, each NULL = not wanted: dx [rows][ld_dx], dgamma / dbeta [c] of gamma's type (no
+ * gamma: dx only, or params' type as params_f32 says).  workspace: gwn_layernorm_bwd_workspace_floats,
+ * needed where dgamma or dbeta is wanted.  dx may be dy (same ld). */
+int gwn_layernorm_bwd(const void* dy, long ld_dy, const void* x, long ldx, long rows, int c, int elem,
+                      const void* gamma, int params_f32, const float* mean, const float* rstd, void* dx, long ld_dx,
+                      void* dgamma, void* dbeta, float* workspace, hipStream_t stream);
+long gwn_layernorm_bwd_workspace_floats(long rows, int c, int elem);
+
+/* y = residual + D(act(z)), z = x w^T + bias: x [M][ldx] (K values a row), w [N][ldw], bias [N] or
+ * NULL, residual [M][ld_res] or NULL, y [M][ldy]; D is gwn_dropout's mask on element m N + n (drop_p
+ * 0 = none, seed_ptr unused).  z [M][ldz] (NULL = no backward follows, or act NONE): the pre-activation
+ * for the backward, float for f32 elements and otherwise f16, saturated, with its sign kept. */
+typedef struct gwn_linear_args {
+  const void* x; long ldx;
+  const void* w; long ldw;
+  const void* bias;
+  const void* residual; long ld_res;
+  void* y; long ldy;
+  void* z; long ldz;
+  int M, N, K;
+  int elem, act;
+  const unsigned long long* seed_ptr; unsigned long long salt; double drop_p;
+  float* workspace; /* gwn_linear_fwd_workspace_floats(M, N, K, elem); may be NULL where that is 0 */
+} gwn_linear_args;
+int gwn_linear_fwd(const gwn_linear_args* a, hipStream_t stream);
+long gwn_linear_fwd_workspace_floats(int M, int N, int K, int elem);
+
+/* Gradients of gwn_linear_fwd, each NULL = not wanted (dresidual is dy itself):
+ *   dz = D'(dy) act'(z) (rounded to the element type where act or dropout make it differ from dy),
+ *   dx = dz w, dw = dz^T x, dbias = sum_m dz (of the unrounded dz).
+ * act, seed, salt and drop_p as the forward had them. */
+typedef struct gwn_linear_bwd_args {
+  const void* dy; long ld_dy;
+  const void* x; long ldx;
+  const void* w; long ldw;
+  const void* z; long ldz;
+  void* dx; long ld_dx;
+  void* dw; long ld_dw;
+  void* dbias;
+  int M, N, K;
+  int elem, act;
+  const unsigned long long* seed_ptr; unsigned long long salt; double drop_p;
+  float* workspace; /* gwn_linear_bwd_workspace_floats(M, N, K, elem), always needed */
+} gwn_linear_bwd_args;
+int gwn_linear_bwd(const gwn_linear_bwd_args* a, hipStream_t stream);
+long gwn_linear_bwd_workspace_floats(int M, int N, int K, int elem);
 
 #ifdef __cplusplus
 }
