@@ -1,176 +1,682 @@
 // y = residual + D(act(x w^T + bias)) in one launch, and its gradients.
 //
 //   z = x w^T + b,  y = r + D(act(z));  dz = D'(dy) act'(z),  db = sum_m dz,  dx = dz w,  dw = dz^T x
+//
+// All three products are one tile kernel whose operands lie either with the contraction contiguous
+// ("K rows": x and w forward, dz for dx) or with the other index contiguous ("M rows": w for dx, dz
+// and x for dw), so that nothing is transposed in memory.
 #include "elem.h"
 
 using namespace elem;
 
 namespace {
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// ---- epilogue -----------------------------------------------------------------------------------
+
 // the saved pre-activation: float beside f32 elements, else f16
 template <typename T> struct ZType { typedef f16 type; };
 template <> struct ZType<float> { typedef float type; };
 
-__device__ __forceinline__ void put_z(float* p, float z) { *p = z; }
-__device__ __forceinline__ void put_z(f16* p, float z) {
+__device__ __forceinline__ float z_of(float z, float) { return z; }
+__device__ __forceinline__ f16 z_of(float z, f16) {
   // finite values stay finite, and a positive one positive: the derivatives' limits and relu's
   // border then come out of the rounded value as out of the exact one
   f16 h = (f16)(fabsf(z) < 3.0e38f ? fminf(fmaxf(z, -65504.0f), 65504.0f) : z);
   if (z > 0.0f && h == (f16)0.0f) h = (f16)5.9604645e-8f;
-  *p = h;
+  return h;
 }
 
 struct Epi {
   const void* bias;
   const void* res; long ld_res;
   void* z; long ldz;
-  int act;
+  void* y; long ldy;
+  int N, act;
   Drop drop;
 };
 
-// C(m, n) = epi(sum_k A[m sam + k sak] B[n sbn + k sbk]), C [M][ldc]
+template <typename T, int V>
+__device__ __forceinline__ void load_f(float (&o)[V], const T* p, int rem) {
+  if (rem >= V) {
+    const Pack<T, V> a = load<T, V>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = (float)a.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = j < rem ? (float)p[j] : 0.0f;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_f(T* p, const float (&v)[V], int rem) {
+  if (rem >= V) {
+    Pack<T, V> a;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.v[j] = (T)v[j];
+    store<T, V>(p, a);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < rem) p[j] = (T)v[j];
+  }
+}
+
+// the mask on elements i .. i + V - 1
+template <int V>
+__device__ __forceinline__ void drop_vec(float (&v)[V], DropKey& key, const Drop& d, unsigned long long i) {
+  key.seek(i);
+  const bool steps = (unsigned)i > 0xFFFFFFFFu - V;  // the high half steps within
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (steps) key.seek(i + j);
+    v[j] = key.keep((unsigned)i + j, d.thr) ? v[j] * d.scale : 0.0f;
+  }
+}
+
+// V columns n .. of row m, of which `rem` lie within N
+template <typename T, int V>
+__device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int n, int rem, float (&v)[V]) {
+  typedef typename ZType<T>::type Z;
+  if (e.bias) {
+    float b[V];
+    load_f<T, V>(b, (const T*)e.bias + n, rem);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += b[j];
+  }
+  if (e.z) {
+    Z* z = (Z*)e.z + m * e.ldz + n;
+    Pack<Z, V> a;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.v[j] = z_of(v[j], Z());
+    if (rem >= V) {
+      store<Z, V>(z, a);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < rem) z[j] = a.v[j];
+    }
+  }
+  if (e.act != GWN_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = act_value<is16<T>>(v[j], e.act);
+  }
+  if (e.drop.thr) drop_vec<V>(v, key, e.drop, (unsigned long long)m * e.N + n);
+  if (e.res) {
+    float r[V];
+    load_f<T, V>(r, (const T*)e.res + m * e.ld_res + n, rem);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += r[j];
+  }
+  store_f<T, V>((T*)e.y + m * e.ldy + n, v, rem);
+}
+
+// ---- the tile kernel ------------------------------------------------------------------------------
+//
+// A workgroup computes BM x BN of C(m, n) = sum_k A(m, k) B(n, k) by v_mfma_f32_32x32x16 (16-bit) or
+// v_mfma_f32_32x32x2_f32, each wave WTM x WTN of it in accumulators.  128 bytes of the contraction a
+// step are staged in LDS by buffer loads that write LDS themselves, 16 bytes a lane, in two
+// buffers: a step's loads are in flight while the step before is multiplied.  LDS is written
+// linearly, so the swizzle that keeps the fragment reads off each other's banks is in the global
+// address: a K row's 16-byte piece c lies at c ^ (row & 7); an M row's (16-bit) at c ^ ((k & 3) << 2),
+// read by ds_read_b64_tr_b16, which hands each lane four k of its own column.  What lies outside
+// the matrices is a load past its buffer resource, which gives zeros.
+// An operand needs 16-byte aligned rows of whole 16-byte pieces; others are copied to such rows first.
+
+enum { K_ROWS = 0, M_ROWS = 1 };
+constexpr unsigned OOR = 0x7ffffff0u;  // past every resource
+constexpr long MAX_LD = 1 << 20;       // rows further apart are copied: offsets within a tile fit 31 bits
+
+struct Operand {
+  const void* p; long ld;
+};
 struct Gemm {
-  const void* A; long sam, sak;
-  const void* B; long sbn, sbk;
-  void* C; long ldc;
-  int M, N, K;
+  Operand a, b;
+  int M, N, K, krows;  // krows: the contraction's rows that M-row operands have (K may count padding)
+  int tiles_m, tiles_n, splits, kchunk;
+  float* part;  // [splits][M][N] (splits > 1)
   Epi e;
 };
 
-template <typename T>
-__device__ __forceinline__ void epilogue(const Gemm& p, DropKey& key, long m, long n, float v) {
-  if (p.e.bias) v += (float)((const T*)p.e.bias)[n];
-  if (p.e.z) put_z((typename ZType<T>::type*)p.e.z + m * p.e.ldz + n, v);
-  v = act_value<is16<T>>(v, p.e.act);
-  if (p.e.drop.thr) {
-    const unsigned long long i = (unsigned long long)m * p.N + n;
-    key.seek(i);
-    v = key.keep((unsigned)i, p.e.drop.thr) ? v * p.e.drop.scale : 0.0f;
-  }
-  if (p.e.res) v += (float)((const T*)p.e.res)[m * p.e.ld_res + n];
-  ((T*)p.C)[m * p.ldc + n] = (T)v;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 rsrc(const void* base, long bytes) {
+  const unsigned long long b = (unsigned long long)base;
+  return u32x4{(unsigned)b, (unsigned)(b >> 32) & 0xffffu, (unsigned)(bytes < 0x7fffff00L ? bytes : 0x7fffff00L),
+               0x00020000u};
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void gemm_kernel(const Gemm p) {
-  __shared__ float As[16][65], Bs[16][65];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const long m0 = (long)blockIdx.x * 64, n0 = (long)blockIdx.y * 64;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    for (int q = threadIdx.x; q < 1024; q += 256) {
-      const int i = p.sak == 1 ? q >> 4 : q & 63, k = p.sak == 1 ? q & 15 : q >> 6;
-      As[k][i] = m0 + i < p.M && k0 + k < p.K ? (float)((const T*)p.A)[(m0 + i) * p.sam + (long)(k0 + k) * p.sak] : 0.0f;
+// 16 bytes a lane from `off` of the resource to LDS at `lds` + 16 lane.  In assembly because the
+// compiler waits for every such load before the next transposed LDS read, whichever buffer either
+// touches; nothing is written to registers, and the loop below waits for vmcnt itself.
+__device__ __forceinline__ void load_lds(u32x4 rs, unsigned off, unsigned lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(off), "s"(rs)
+      : "memory");  // m0 is reserved: the compiler sets it before each use of its own, and has none here
+}
+
+// R rows (or columns) of an operand, one step of 128 bytes of k, by NT threads
+template <typename T, int L, int R, int NT>
+struct Stage {
+  static constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
+  static constexpr int PER = R * 8 / NT, CPR = R * (int)sizeof(T) / 16;
+  static_assert(R * 8 % NT == 0, "whole loads");
+  unsigned off[PER];
+  int k;  // K rows: this thread's k within a step
+  __device__ __forceinline__ void init(const Operand& o, int r0, int rows) {
+    const int tid = threadIdx.x;
+    const unsigned ldb = (unsigned)(o.ld * (long)sizeof(T));
+    if (L == K_ROWS) {
+      const int c = (tid & 7) ^ ((tid >> 3) & 7);
+      k = c * E;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r = i * (NT / 8) + (tid >> 3);
+        off[i] = r0 + r < rows ? r * ldb + c * 16 : OOR;
+      }
+    } else {
+      k = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int q = i * NT + tid, kk = q / CPR;
+        const int c = (q % CPR) ^ (sizeof(T) == 2 ? (kk & 3) << 2 : 0);
+        off[i] = r0 + c * E < rows ? kk * ldb + c * 16 : OOR;
+      }
     }
-    for (int q = threadIdx.x; q < 1024; q += 256) {
-      const int i = p.sbk == 1 ? q >> 4 : q & 63, k = p.sbk == 1 ? q & 15 : q >> 6;
-      Bs[k][i] = n0 + i < p.N && k0 + k < p.K ? (float)((const T*)p.B)[(n0 + i) * p.sbn + (long)(k0 + k) * p.sbk] : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += As[k][ty * 4 + i] * Bs[k][tx + 16 * j];
-    __syncthreads();
   }
+  // step k0 .. of this operand into LDS at `to`; kend: the contraction's end
+  __device__ __forceinline__ void load(const Operand& o, int r0, int rows, int k0, int kend, int krows, unsigned to,
+                                       int wave) const {
+    const long ld = o.ld;
+    u32x4 rs;
+    bool ok = true;
+    if (L == K_ROWS) {
+      const int nr = rows - r0 < R ? rows - r0 : R;
+      rs = rsrc((const T*)o.p + (long)r0 * ld + k0, ((long)(nr - 1) * ld + (kend - k0)) * (long)sizeof(T));
+      ok = k0 + k < kend;
+    } else {
+      const int left = (kend < krows ? kend : krows) - k0, nk = left < BK ? left : BK;
+      rs = rsrc((const T*)o.p + (long)k0 * ld + r0, ((long)(nk - 1) * ld + (rows - r0 + E - 1) / E * E) * (long)sizeof(T));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) load_lds(rs, ok ? off[i] : OOR, to + (i * NT + wave * 64) * 16);
+  }
+};
+
+// the fragments of one 32-row tile for 16 contraction values (16-bit)
+template <typename T, int L, int R>
+__device__ __forceinline__ s16x8 frag16(const char* s, int row0, int ks, int lane) {
+  if (L == K_ROWS) {
+    const int row = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
+    return *(const s16x8*)(s + row * 128 + ((c ^ (row & 7)) << 4));
+  }
+  const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
+  const int col = row0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+  const char* at = s + k * (R * 2) + (((col >> 3) ^ ((k & 3) << 2)) << 4) + (col & 7) * 2;
+  typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 4 * R * 2));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// four contraction values of one 32-row tile: k = 4 (2 q + lane / 32) + 0 .. 3 (f32)
+template <int L, int R>
+__device__ __forceinline__ f32x4 frag32(const char* s, int row0, int q, int lane) {
+  const int row = row0 + (lane & 31), c = q * 2 + (lane >> 5);
+  if (L == K_ROWS) return *(const f32x4*)(s + row * 128 + ((c ^ (row & 7)) << 4));
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = *(const float*)(s + (c * 4 + e) * (R * 4) + row * 4);
+  return v;
+}
+
+__device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+__device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, f16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// workgroup -> (tile, split).  Consecutive workgroups go to the 8 XCDs in turn: each XCD gets a
+// contiguous run of tiles, 8 rows of tiles walked column by column, so that its L2 holds the operands
+// they share.
+__device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& split) {
+  const int total = gridDim.x, per = total >> 3;
+  int id = blockIdx.x;
+  if (id < per * 8) id = (id & 7) * per + (id >> 3);
+  const int tiles = p.tiles_m * p.tiles_n;
+  split = id / tiles;
+  id -= split * tiles;
+  const int width = 8 * p.tiles_n, g = id / width, first = g * 8;
+  const int rows = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
+  id -= g * width;
+  tn = id / rows;
+  tm = first + id - tn * rows;
+}
+
+template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN>
+__global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
+  constexpr int NT = 64 * WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 32, TN = WTN / 32;
+  constexpr int BK = 128 / (int)sizeof(T), STAGE = (BM + BN) * 128;
+  constexpr int EW = WTN + 4;  // floats a row of the epilogue's image of one wave's 32 rows
+  constexpr int SMEM = 2 * STAGE > WGM * WGN * 32 * EW * 4 ? 2 * STAGE : WGM * WGN * 32 * EW * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WGM, wn = wave / WGM;
+  const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)smem;
+  int tm, tn, split;
+  place(p, tm, tn, split);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int kbeg = split * p.kchunk, kend = p.K - kbeg < p.kchunk ? p.K : kbeg + p.kchunk;
+
+  Stage<T, LA, BM, NT> sa;
+  Stage<T, LB, BN, NT> sb;
+  sa.init(p.a, m0, p.M);
+  sb.init(p.b, n0, p.N);
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  auto issue = [&](int k0, int buf) {
+    sa.load(p.a, m0, p.M, k0, kend, p.krows, lds0 + buf * STAGE, wave);
+    sb.load(p.b, n0, p.N, k0, kend, p.krows, lds0 + buf * STAGE + BM * 128, wave);
+  };
+  if (kbeg < kend) issue(kbeg, 0);
+  int buf = 0;
+  for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
+    // this wave's loads of the step have landed; behind the barrier every wave's have, and every wave
+    // has read the other buffer for the last time
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (k0 + BK < kend) issue(k0 + BK, buf ^ 1);
+    const char* A = smem + buf * STAGE;
+    const char* B = A + BM * 128;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if constexpr (sizeof(T) == 2) {
+        s16x8 fa[TM], fb[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[i] = frag16<T, LA, BM>(A, wm * WTM + i * 32, ks, lane);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[j] = frag16<T, LB, BN>(B, wn * WTN + j * 32, ks, lane);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = mma(fa[i], fb[j], acc[i][j], T());
+      } else {
+        f32x4 fa[TM], fb[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[i] = frag32<LA, BM>(A, wm * WTM + i * 32, ks, lane);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[j] = frag32<LB, BN>(B, wn * WTN + j * 32, ks, lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i][e], fb[j][e], acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+
+  // 32 rows of a wave at a time through LDS, from the accumulators' layout to whole row pieces
+  __syncthreads();
+  constexpr int V = 16 / (int)sizeof(T), LPR = WTN / V, RPI = 64 / LPR;
+  float* img = (float*)smem + wave * 32 * EW;
   DropKey key;
   if (p.e.drop.thr) key.init(p.e.drop, (unsigned long long)m0 * p.N + n0);
+  const int n = n0 + wn * WTN + (lane % LPR) * V, rem = p.N - n;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < TM; ++i) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-      if (m < p.M && n < p.N) epilogue<T>(p, key, m, n, acc[i][j]);
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        img[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * EW + j * 32 + (lane & 31)] = acc[i][j][r];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int q = 0; q < 32 / RPI; ++q) {
+      const int row = q * RPI + lane / LPR;
+      const long m = m0 + wm * WTM + i * 32 + row;
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = img[row * EW + (lane % LPR) * V + j];
+      if (m < p.M && rem > 0) {
+        if (p.splits > 1)
+          store_f<float, V>(p.part + ((long)split * p.M + m) * p.N + n, v, rem);
+        else
+          epilogue<T, V>(p.e, key, m, n, rem, v);
+      }
     }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
+// the splits' sums, in their order, and the epilogue: V columns a thread
 template <typename T>
-int gemm(const Gemm& p, hipStream_t s) {
-  gemm_kernel<T><<<dim3((p.M + 63) / 64, (p.N + 63) / 64), 256, 0, s>>>(p);
-  GWN_CHECK_LAUNCH();
-  return GWN_OK;
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int M, int N, Epi e) {
+  constexpr int V = 4;
+  const long per = (N + V - 1) / V, total = per * M;
+  DropKey key;
+  if (e.drop.thr) key.init(e.drop, (unsigned long long)blockIdx.x * 256 * V);
+  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
+    const long m = q / per;
+    const int n = (int)(q - m * per) * V, rem = N - n;
+    const float* at = part + m * N + n;
+    float v[V] = {};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      float o[V];
+      load_f<float, V>(o, at + (long)s * M * N, rem);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += o[j];
+    }
+    epilogue<T, V>(e, key, m, n, rem, v);
+  }
 }
+
+// rows [rows][ld] -> [rows][ldo] with zeros past `cols`: a 16-byte piece a thread
+template <typename T>
+__global__ __launch_bounds__(256) void copy_rows_kernel(const T* x, long ld, long rows, int cols, T* o, int ldo) {
+  constexpr int V = Vec<T>::N;
+  const int per = ldo / V;
+  const long total = rows * per;
+  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
+    const long m = q / per;
+    const int n = (int)(q - m * per) * V, rem = cols - n;
+    Pack<T, V> a;
+    if (rem >= V) {
+      a = load<T, V>(x + m * ld + n);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) a.v[j] = j < rem ? x[m * ld + n + j] : (T)0.0f;
+    }
+    store<T, V>(o + m * ldo + n, a);
+  }
+}
+
+// ---- dz and the bias's gradient -------------------------------------------------------------------
 
 struct Dz {
   const void* dy; long ld_dy;
   const void* z; long ldz;
-  void* dz;     // [M][N], NULL = not written (dz is dy)
-  float* part;  // [gridDim.y][N] column sums, NULL = not wanted
+  void* dz; int ld;  // [M][ld], columns past N zero; NULL = not written
+  float* part;       // [gridDim.y][N] column sums, NULL = not wanted
   int M, N, act;
   Drop drop;
 };
 
-// 256 columns x a stripe of rows a workgroup
-template <typename T>
+// TX pieces of 16 bytes of columns x 256 / TX rows a workgroup, rows split over gridDim.y; each
+// thread sums its columns in fp32 before dz is rounded.  Bound by memory: dy and z read, dz written.
+template <typename T, int TX>
 __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
-  const long n = (long)blockIdx.x * 256 + threadIdx.x;
-  if (n >= p.N) return;
+  typedef typename ZType<T>::type Z;
+  constexpr int V = Vec<T>::N, TY = 256 / TX;
+  __shared__ float cols[TY][TX * V + 1];
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const long n = ((long)blockIdx.x * TX + tx) * V;
+  const int rem = (int)(p.N - n < V ? p.N - n : V);
+  float sum[V] = {};
   DropKey key;
-  if (p.drop.thr) key.init(p.drop, (unsigned long long)blockIdx.y * p.N);
-  float sum = 0.0f;
-  for (long m = blockIdx.y; m < p.M; m += gridDim.y) {
-    float v = (float)((const T*)p.dy)[m * p.ld_dy + n];
-    if (p.drop.thr) {
-      const unsigned long long i = (unsigned long long)m * p.N + n;
-      key.seek(i);
-      v = key.keep((unsigned)i, p.drop.thr) ? v * p.drop.scale : 0.0f;
+  if (p.drop.thr) key.init(p.drop, (unsigned long long)blockIdx.y * TY * p.N);
+  if (rem > 0)
+    for (long m = (long)blockIdx.y * TY + ty; m < p.M; m += (long)gridDim.y * TY) {
+      float v[V];
+      load_f<T, V>(v, (const T*)p.dy + m * p.ld_dy + n, rem);
+      if (p.drop.thr) drop_vec<V>(v, key, p.drop, (unsigned long long)m * p.N + n);
+      if (p.act != GWN_ACT_NONE) {
+        float z[V];
+        load_f<Z, V>(z, (const Z*)p.z + m * p.ldz + n, rem);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] *= act_slope<is16<T>>(z[j], p.act);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (j >= rem) v[j] = 0.0f;
+        sum[j] += v[j];
+      }
+      if (p.dz) store_f<T, V>((T*)p.dz + m * p.ld + n, v, V);
     }
-    if (p.act != GWN_ACT_NONE)
-      v *= act_slope<is16<T>>((float)((const typename ZType<T>::type*)p.z)[m * p.ldz + n], p.act);
-    sum += v;
-    if (p.dz) ((T*)p.dz)[m * p.N + n] = (T)v;
+  if (!p.part) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) cols[ty][tx * V + j] = sum[j];
+  __syncthreads();
+  for (int k = threadIdx.x; k < TX * V; k += 256) {
+    const long at = (long)blockIdx.x * TX * V + k;
+    if (at < p.N) {
+      float v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < TY; ++q) v += cols[q][k];
+      p.part[(long)blockIdx.y * p.N + at] = v;
+    }
   }
-  if (p.part) p.part[(long)blockIdx.y * p.N + n] = sum;
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void colsum_kernel(const float* part, int nparts, int n, T* out) {
-  const long k = (long)blockIdx.x * 256 + threadIdx.x;
-  if (k >= n) return;
+__global__ __launch_bounds__(1024) void colsum_kernel(const float* part, int nparts, int n, T* out) {
+  __shared__ float s[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long k = (long)blockIdx.x * 32 + tx;
   float v = 0.0f;
-  for (int q = 0; q < nparts; ++q) v += part[(long)q * n + k];
-  out[k] = (T)v;
+  if (k < n)
+#pragma unroll 8
+    for (int q = ty; q < nparts; q += 32) v += part[(long)q * n + k];
+  s[ty][tx] = v;
+  __syncthreads();
+  if (ty == 0 && k < n) {
+    v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v += s[q][tx];
+    out[k] = (T)v;
+  }
 }
 
-int dz_parts(int M) { return M < 1 ? 1 : M < 256 ? M : 256; }
+// ---- plans ------------------------------------------------------------------------------------------
+
+long up(long v, long to) { return (v + to - 1) / to * to; }
+int vec_of(int elem) { return 16 / elem_bytes(elem); }
+
+// whether rows of `cols` values can be staged where they lie
+bool stageable(const void* p, long ld, int cols, int elem) {
+  const int v = vec_of(elem);
+  return ((size_t)p & 15) == 0 && ld % v == 0 && ld <= MAX_LD && cols % v == 0;
+}
+// floats of a copy with whole pieces a row
+long copy_floats(long rows, int cols, int elem) { return up(rows * up(cols, vec_of(elem)) * elem_bytes(elem), 16) / 4; }
+
+struct Shape { int bm, bn, tiles_m, tiles_n, splits, kchunk; };
+
+Shape shape_of(int M, int N, int K, int elem) {
+  Shape s;
+  const long cus = gwn_device_cus();
+  const bool big = elem != GWN_ELEM_F32 && ((M + 255L) / 256) * ((N + 255L) / 256) >= cus;
+  s.bm = s.bn = big ? 256 : 128;
+  s.tiles_m = (M + s.bm - 1) / s.bm;
+  s.tiles_n = (N + s.bn - 1) / s.bn;
+  const long tiles = (long)s.tiles_m * s.tiles_n;
+  const int bk = 128 / elem_bytes(elem);
+  const long steps = (K + bk - 1) / bk;
+  long splits = 1;
+  if (tiles < cus) {
+    splits = (2 * cus) / tiles;
+    if (splits > steps / 4) splits = steps / 4;
+    if (splits < 1) splits = 1;
+  }
+  s.kchunk = (int)((steps + splits - 1) / splits) * bk;
+  s.splits = K ? (K + s.kchunk - 1) / s.kchunk : 1;
+  if (s.splits < 1) s.splits = 1;
+  return s;
+}
+long part_floats(int M, int N, int K, int elem) {
+  const Shape s = shape_of(M, N, K, elem);
+  return s.splits > 1 ? up((long)s.splits * M * N, 4) : 0;
+}
+
+template <typename T>
+int gemm(int la, int lb, Operand a, Operand b, int M, int N, int K, int krows, int elem, const Epi& e, float* part,
+         hipStream_t s) {
+  const Shape sh = shape_of(M, N, K, elem);
+  const long tiles = (long)sh.tiles_m * sh.tiles_n * sh.splits;
+  GWN_REQUIRE(tiles < (1L << 22), "linear: too many tiles for one launch");
+  Gemm p{a, b, M, N, K, krows, sh.tiles_m, sh.tiles_n, sh.splits, sh.kchunk, part, e};
+  const int grid = (int)tiles;
+  if constexpr (sizeof(T) == 2) {
+    if (sh.bm == 256) {
+      if (la == K_ROWS && lb == K_ROWS)
+        gemm_kernel<T, K_ROWS, K_ROWS, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
+      else if (la == K_ROWS)
+        gemm_kernel<T, K_ROWS, M_ROWS, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
+      else
+        gemm_kernel<T, M_ROWS, M_ROWS, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
+    }
+  }
+  if (sh.bm == 128) {
+    if (la == K_ROWS && lb == K_ROWS)
+      gemm_kernel<T, K_ROWS, K_ROWS, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
+    else if (la == K_ROWS)
+      gemm_kernel<T, K_ROWS, M_ROWS, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
+    else
+      gemm_kernel<T, M_ROWS, M_ROWS, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
+  }
+  GWN_CHECK_LAUNCH();
+  if (sh.splits > 1) {
+    const long want = ((long)M * ((N + 3) / 4) + 255) / 256, most = (long)gwn_device_cus() * 16;
+    join_kernel<T><<<(int)(want < most ? want : most), 256, 0, s>>>(part, sh.splits, M, N, e);
+    GWN_CHECK_LAUNCH();
+  }
+  return GWN_OK;
+}
+
+template <typename T>
+int copy_rows(const void* x, long ld, long rows, int cols, float*& at, int elem, Operand& o, hipStream_t s) {
+  const int ldo = (int)up(cols, vec_of(elem));
+  const long want = (rows * (ldo / vec_of(elem)) + 255) / 256, most = (long)gwn_device_cus() * 16;
+  copy_rows_kernel<T><<<(int)(want < most ? want : most), 256, 0, s>>>((const T*)x, ld, rows, cols, (T*)at, ldo);
+  GWN_CHECK_LAUNCH();
+  o = {at, ldo};
+  at += copy_floats(rows, cols, elem);
+  return GWN_OK;
+}
+
+long fwd_floats(const gwn_linear_args* a) {
+  long f = part_floats(a->M, a->N, a->K, a->elem);
+  if (!stageable(a->x, a->ldx, a->K, a->elem)) f += copy_floats(a->M, a->K, a->elem);
+  if (!stageable(a->w, a->ldw, a->K, a->elem)) f += copy_floats(a->N, a->K, a->elem);
+  return f;
+}
 
 template <typename T>
 int fwd(const gwn_linear_args* a, hipStream_t s) {
-  Gemm p{a->x, a->ldx, 1, a->w, a->ldw, 1, a->y, a->ldy, a->M, a->N, a->K, {}};
-  p.e = {a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->act,
-         drop_of(a->seed_ptr, a->salt, a->drop_p)};
-  return gemm<T>(p, s);
+  Operand x{a->x, a->ldx}, w{a->w, a->ldw};
+  float* at = a->workspace;
+  if (!stageable(a->x, a->ldx, a->K, a->elem)) {
+    const int rc = copy_rows<T>(a->x, a->ldx, a->M, a->K, at, a->elem, x, s);
+    if (rc) return rc;
+  }
+  if (!stageable(a->w, a->ldw, a->K, a->elem)) {
+    const int rc = copy_rows<T>(a->w, a->ldw, a->N, a->K, at, a->elem, w, s);
+    if (rc) return rc;
+  }
+  const Epi e{a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->y, a->ldy, a->N, a->act,
+              drop_of(a->seed_ptr, a->salt, a->drop_p)};
+  const int kp = (int)up(a->K, vec_of(a->elem));  // a copy's zeros included
+  return gemm<T>(K_ROWS, K_ROWS, x, w, a->M, a->N, kp, kp, a->elem, e, at, s);
+}
+
+struct BwdPlan {
+  bool write_dz, copy_x, copy_w;  // dz apart from dy; operands that have to be copied
+  int parts, tx, ld_dz;
+  long floats;
+};
+BwdPlan bwd_plan(const gwn_linear_bwd_args* a) {
+  BwdPlan q;
+  const int v = vec_of(a->elem);
+  const bool product = (a->dx || a->dw) && a->M;
+  q.write_dz = product && (a->act != GWN_ACT_NONE || a->drop_p > 0.0 || !stageable(a->dy, a->ld_dy, a->N, a->elem));
+  q.copy_x = a->dw && a->M && !stageable(a->x, a->ldx, a->K, a->elem);
+  q.copy_w = a->dx && a->M && !stageable(a->w, a->ldw, a->K, a->elem);
+  q.ld_dz = (int)up(a->N, v);
+  const int pieces = q.ld_dz / v;
+  q.tx = pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : 64;
+  const long bx = (pieces + q.tx - 1) / q.tx, ty = 256 / q.tx;
+  long parts = (8L * gwn_device_cus() + bx - 1) / bx, most = (a->M + 4 * ty - 1) / (4 * ty);
+  if (parts > most) parts = most;
+  if (parts > 1024) parts = 1024;
+  q.parts = (int)(parts < 1 ? 1 : parts);
+  q.floats = a->dbias ? up((long)q.parts * a->N, 4) : 0;
+  if (q.write_dz) q.floats += copy_floats(a->M, a->N, a->elem);
+  if (q.copy_x) q.floats += copy_floats(a->M, a->K, a->elem);
+  if (q.copy_w) q.floats += copy_floats(a->N, a->K, a->elem);
+  long part = 0;
+  if (a->dx && a->M) part = part_floats(a->M, a->K, q.ld_dz, a->elem);
+  if (a->dw) {
+    const long f = part_floats(a->N, a->K, a->M, a->elem);
+    if (f > part) part = f;
+  }
+  q.floats += part;
+  return q;
 }
 
 template <typename T>
 int bwd(const gwn_linear_bwd_args* a, hipStream_t s) {
+  const BwdPlan q = bwd_plan(a);
   const Drop drop = drop_of(a->seed_ptr, a->salt, a->drop_p);
-  const bool changes = a->act != GWN_ACT_NONE || drop.thr;
-  const bool product = a->dx || a->dw;
-  const int parts = dz_parts(a->M);
-  T* dzbuf = (T*)(a->workspace + (long)parts * a->N);
-  const T* dz = changes ? dzbuf : (const T*)a->dy;
-  const long ld = changes ? a->N : a->ld_dy;
-  if ((changes && product) || a->dbias) {
-    const Dz q{a->dy, a->ld_dy, a->z, a->ldz, changes && product ? dzbuf : nullptr, a->dbias ? a->workspace : nullptr,
-               a->M, a->N, a->act, drop};
-    dz_kernel<T><<<dim3((a->N + 255) / 256, parts), 256, 0, s>>>(q);
+  float* at = a->workspace;
+  float* sums = at;
+  if (a->dbias) at += up((long)q.parts * a->N, 4);
+  Operand dz{a->dy, a->ld_dy}, x{a->x, a->ldx}, w{a->w, a->ldw};
+  if (q.write_dz) {
+    dz = {at, q.ld_dz};
+    at += copy_floats(a->M, a->N, a->elem);
+  }
+  if (q.write_dz || a->dbias) {
+    const Dz d{a->dy, a->ld_dy, a->z, a->ldz, q.write_dz ? (void*)dz.p : nullptr, q.ld_dz, a->dbias ? sums : nullptr, a->M,
+               a->N, a->act, drop};
+    const dim3 grid((q.ld_dz / vec_of(a->elem) + q.tx - 1) / q.tx, q.parts);
+    if (q.tx == 8) dz_kernel<T, 8><<<grid, 256, 0, s>>>(d);
+    if (q.tx == 16) dz_kernel<T, 16><<<grid, 256, 0, s>>>(d);
+    if (q.tx == 32) dz_kernel<T, 32><<<grid, 256, 0, s>>>(d);
+    if (q.tx == 64) dz_kernel<T, 64><<<grid, 256, 0, s>>>(d);
     GWN_CHECK_LAUNCH();
   }
   if (a->dbias) {
-    colsum_kernel<T><<<(a->N + 255) / 256, 256, 0, s>>>(a->workspace, parts, a->N, (T*)a->dbias);
+    colsum_kernel<T><<<(a->N + 31) / 32, 1024, 0, s>>>(sums, q.parts, a->N, (T*)a->dbias);
     GWN_CHECK_LAUNCH();
   }
+  int rc = GWN_OK;
+  if (q.copy_x && (rc = copy_rows<T>(a->x, a->ldx, a->M, a->K, at, a->elem, x, s))) return rc;
+  if (q.copy_w && (rc = copy_rows<T>(a->w, a->ldw, a->N, a->K, at, a->elem, w, s))) return rc;
+  Epi e{};
   if (a->dx && a->M) {
-    Gemm p{dz, ld, 1, a->w, 1, a->ldw, a->dx, a->ld_dx, a->M, a->K, a->N, {}};
-    const int rc = gemm<T>(p, s);
+    e.y = a->dx, e.ldy = a->ld_dx, e.N = a->K;
+    // the contraction over N takes dz's padding in; w has N rows, past them its resource gives zeros
+    rc = gemm<T>(K_ROWS, M_ROWS, dz, w, a->M, a->K, q.ld_dz, a->N, a->elem, e, at, s);
     if (rc) return rc;
   }
   if (a->dw) {
-    Gemm p{dz, 1, ld, a->x, 1, a->ldx, a->dw, a->ld_dw, a->N, a->K, a->M, {}};
-    const int rc = gemm<T>(p, s);
+    e.y = a->dw, e.ldy = a->ld_dw, e.N = a->K;
+    rc = gemm<T>(M_ROWS, M_ROWS, dz, x, a->N, a->K, a->M, a->M, a->elem, e, at, s);
     if (rc) return rc;
   }
   return GWN_OK;
@@ -182,7 +688,7 @@ int shape_checks(int M, int N, int K, int elem, int act, double drop_p, const vo
   GWN_REQUIRE(elem_ok(elem), "linear: unknown element type");
   GWN_REQUIRE(act >= GWN_ACT_NONE && act <= GWN_ACT_SILU, "linear: unknown activation");
   GWN_REQUIRE(M >= 0 && N > 0 && K > 0, "linear: M must be >= 0, N and K > 0");
-  GWN_REQUIRE(M <= (1 << 30) && N <= (1 << 21) && K <= (1 << 21), "linear: M is at most 2^30, N and K 2^21");
+  GWN_REQUIRE(M <= (1 << 30) && N <= MAX_LD && K <= MAX_LD, "linear: M is at most 2^30, N and K 2^20");
   GWN_REQUIRE(drop_p >= 0.0 && drop_p <= 1.0, "linear: the dropout rate must be between 0 and 1");
   GWN_REQUIRE(drop_p == 0.0 || (seed_ptr && ((size_t)seed_ptr & 7) == 0), "linear: dropout needs a seed");
   return GWN_OK;
@@ -192,9 +698,9 @@ int shape_checks(int M, int N, int K, int elem, int act, double drop_p, const vo
 
 extern "C" {
 
-long gwn_linear_fwd_workspace_floats(int M, int N, int K, int elem) {
-  (void)M, (void)N, (void)K, (void)elem;
-  return 0;
+long gwn_linear_fwd_workspace_floats(const gwn_linear_args* a) {
+  if (!a || shape_checks(a->M, a->N, a->K, a->elem, a->act, a->drop_p, a->seed_ptr) || a->M == 0) return 0;
+  return fwd_floats(a);
 }
 
 int gwn_linear_fwd(const gwn_linear_args* a, hipStream_t stream) {
@@ -210,7 +716,7 @@ int gwn_linear_fwd(const gwn_linear_args* a, hipStream_t stream) {
   GWN_REQUIRE((((size_t)a->x | (size_t)a->w | (size_t)a->bias | (size_t)a->residual | (size_t)a->y | (size_t)a->z) &
                (e - 1)) == 0,
               "linear: a pointer is not aligned to its element");
-  const long ws = gwn_linear_fwd_workspace_floats(a->M, a->N, a->K, a->elem);
+  const long ws = fwd_floats(a);
   GWN_REQUIRE(ws == 0 || (a->workspace && ((size_t)a->workspace & 15) == 0), "linear: the workspace is missing");
   GWN_DEBUG_RANGE(a->x, range_bytes(a->M, a->ldx, a->K, e), "linear x");
   GWN_DEBUG_RANGE(a->w, range_bytes(a->N, a->ldw, a->K, e), "linear w");
@@ -223,9 +729,9 @@ int gwn_linear_fwd(const gwn_linear_args* a, hipStream_t stream) {
   return fwd<bf16>(a, stream);
 }
 
-long gwn_linear_bwd_workspace_floats(int M, int N, int K, int elem) {
-  if (M < 0 || N <= 0 || K <= 0 || !elem_ok(elem)) return 0;
-  return (long)dz_parts(M) * N + ((long)M * N * elem_bytes(elem) + 3) / 4;
+long gwn_linear_bwd_workspace_floats(const gwn_linear_bwd_args* a) {
+  if (!a || shape_checks(a->M, a->N, a->K, a->elem, a->act, a->drop_p, a->seed_ptr)) return 0;
+  return bwd_plan(a).floats;
 }
 
 int gwn_linear_bwd(const gwn_linear_bwd_args* a, hipStream_t stream) {
@@ -244,7 +750,8 @@ int gwn_linear_bwd(const gwn_linear_bwd_args* a, hipStream_t stream) {
   GWN_REQUIRE((((size_t)a->dy | (size_t)a->x | (size_t)a->w | (size_t)a->z | (size_t)a->dx | (size_t)a->dw |
                 (size_t)a->dbias) & (e - 1)) == 0,
               "linear_bwd: a pointer is not aligned to its element");
-  GWN_REQUIRE(a->workspace && ((size_t)a->workspace & 15) == 0, "linear_bwd: the workspace is missing");
+  const long ws = bwd_plan(a).floats;
+  GWN_REQUIRE(ws == 0 || (a->workspace && ((size_t)a->workspace & 15) == 0), "linear_bwd: the workspace is missing");
   GWN_DEBUG_RANGE(a->dy, range_bytes(a->M, a->ld_dy, a->N, e), "linear_bwd dy");
   if (a->dw) GWN_DEBUG_RANGE(a->x, range_bytes(a->M, a->ldx, a->K, e), "linear_bwd x");
   if (a->dx) GWN_DEBUG_RANGE(a->w, range_bytes(a->N, a->ldw, a->K, e), "linear_bwd w");
@@ -252,7 +759,7 @@ int gwn_linear_bwd(const gwn_linear_bwd_args* a, hipStream_t stream) {
     GWN_DEBUG_RANGE(a->z, range_bytes(a->M, a->ldz, a->N, a->elem == GWN_ELEM_F32 ? 4 : 2), "linear_bwd z");
   GWN_DEBUG_RANGE(a->dx, range_bytes(a->M, a->ld_dx, a->K, e), "linear_bwd dx");
   GWN_DEBUG_RANGE(a->dw, range_bytes(a->N, a->ld_dw, a->K, e), "linear_bwd dw");
-  GWN_DEBUG_RANGE(a->workspace, gwn_linear_bwd_workspace_floats(a->M, a->N, a->K, a->elem) * 4, "linear_bwd workspace");
+  GWN_DEBUG_RANGE(a->workspace, ws * 4, "linear_bwd workspace");
   if (a->elem == GWN_ELEM_F32) return bwd<float>(a, stream);
   if (a->elem == GWN_ELEM_F16) return bwd<f16>(a, stream);
   return bwd<bf16>(a, stream);

@@ -335,9 +335,9 @@ _SIGS = [
                                   c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p]),
     ("gwn_layernorm_bwd_workspace_floats", c_long, [c_long, c_int, c_int]),
     ("gwn_linear_fwd", c_int, [ctypes.POINTER(LinearArgs), c_void_p]),
-    ("gwn_linear_fwd_workspace_floats", c_long, [c_int, c_int, c_int, c_int]),
+    ("gwn_linear_fwd_workspace_floats", c_long, [ctypes.POINTER(LinearArgs)]),
     ("gwn_linear_bwd", c_int, [ctypes.POINTER(LinearBwdArgs), c_void_p]),
-    ("gwn_linear_bwd_workspace_floats", c_long, [c_int, c_int, c_int, c_int]),
+    ("gwn_linear_bwd_workspace_floats", c_long, [ctypes.POINTER(LinearBwdArgs)]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]

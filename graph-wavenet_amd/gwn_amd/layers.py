@@ -110,7 +110,7 @@ def _linear_fwd(x, weight, bias, act, residual, p, seed, salt, keep_z):
     if p > 0.0:
         a.seed_ptr, a.salt, a.drop_p = seed.data_ptr(), salt, p
     with _on(x):
-        ws = _ws(_lib.load().gwn_linear_fwd_workspace_floats(m, n, k, a.elem), x.device)
+        ws = _ws(_lib.load().gwn_linear_fwd_workspace_floats(ctypes.byref(a)), x.device)
         a.workspace = _lib.ptr(ws)
         _lib.call("gwn_linear_fwd", ctypes.byref(a), _lib.stream())
     return y, z
@@ -156,7 +156,7 @@ class _LinearActFn(torch.autograd.Function):
         if seed is not None:
             a.seed_ptr, a.salt, a.drop_p = seed.data_ptr(), ctx.salt, ctx.p
         with _on(dy):
-            ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(m, n, k, a.elem), dev)
+            ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(ctypes.byref(a)), dev)
             a.workspace = _lib.ptr(ws)
             _lib.call("gwn_linear_bwd", ctypes.byref(a), _lib.stream())
         return dx, dw, db, dres, None, None, None, None

@@ -810,10 +810,11 @@ typedef struct gwn_linear_args {
   int M, N, K;
   int elem, act;
   const unsigned long long* seed_ptr; unsigned long long salt; double drop_p;
-  float* workspace; /* gwn_linear_fwd_workspace_floats(M, N, K, elem); may be NULL where that is 0 */
+  float* workspace; /* gwn_linear_fwd_workspace_floats floats, 16-byte aligned; may be NULL where that is 0 */
 } gwn_linear_args;
 int gwn_linear_fwd(const gwn_linear_args* a, hipStream_t stream);
-long gwn_linear_fwd_workspace_floats(int M, int N, int K, int elem);
+/* of a call with these arguments, their workspace aside (0 for sizes that the call refuses) */
+long gwn_linear_fwd_workspace_floats(const gwn_linear_args* a);
 
 /* Gradients of gwn_linear_fwd, each NULL = not wanted (dresidual is dy itself):
  *   dz = D'(dy) act'(z) (rounded to the element type where act or dropout make it differ from dy),
@@ -830,10 +831,10 @@ typedef struct gwn_linear_bwd_args {
   int M, N, K;
   int elem, act;
   const unsigned long long* seed_ptr; unsigned long long salt; double drop_p;
-  float* workspace; /* gwn_linear_bwd_workspace_floats(M, N, K, elem), always needed */
+  float* workspace; /* gwn_linear_bwd_workspace_floats floats, 16-byte aligned; may be NULL where that is 0 */
 } gwn_linear_bwd_args;
 int gwn_linear_bwd(const gwn_linear_bwd_args* a, hipStream_t stream);
-long gwn_linear_bwd_workspace_floats(int M, int N, int K, int elem);
+long gwn_linear_bwd_workspace_floats(const gwn_linear_bwd_args* a);
 
 #ifdef __cplusplus
 }

@@ -25,7 +25,7 @@ def linear_args(lib_mod, cls, **kw):
                                 dict(drop_p=float("nan"), seed_ptr=PTR), dict(drop_p=0.5, seed_ptr=PTR + 4), dict(x=None),
                                 dict(w=None), dict(y=None), dict(ldx=15), dict(ldw=15), dict(ldy=7), dict(x=PTR + 1),
                                 dict(w=PTR + 1), dict(y=PTR + 1), dict(residual=PTR, ld_res=7), dict(z=PTR, ldz=7),
-                                dict(residual=PTR + 1, ld_res=8), dict(M=(1 << 30) + 1), dict(N=(1 << 21) + 1)])
+                                dict(residual=PTR + 1, ld_res=8), dict(M=(1 << 30) + 1), dict(N=(1 << 20) + 1)])
 def test_linear_fwd_refuses(kw):
     from gwn_amd import _lib
     with pytest.raises(_lib.GwnError, match="linear"):
@@ -33,8 +33,8 @@ def test_linear_fwd_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(N=0), dict(K=0), dict(elem=7), dict(act=9), dict(drop_p=0.5), dict(dy=None),
-                                dict(x=None), dict(w=None), dict(act=2, z=None), dict(workspace=None),
-                                dict(workspace=PTR + 4), dict(ld_dy=7), dict(ldx=15), dict(ldw=15), dict(act=2, ldz=7),
+                                dict(x=None), dict(w=None), dict(act=2, z=None), dict(act=1, workspace=None),
+                                dict(act=1, workspace=PTR + 4), dict(ld_dy=7), dict(ldx=15), dict(ldw=15), dict(act=2, ldz=7),
                                 dict(ld_dx=15), dict(ld_dw=15), dict(dy=PTR + 1), dict(dw=PTR + 1)])
 def test_linear_bwd_refuses(kw):
     from gwn_amd import _lib
@@ -106,8 +106,14 @@ def test_workspace_sizes():
     for m in (0, 1, 300, 20000, 1 << 29):
         for n, k in ((1, 1), (33, 70), (8192, 2048)):
             for elem, size in ((0, 4), (1, 2), (2, 2)):
-                assert lib.gwn_linear_bwd_workspace_floats(m, n, k, elem) * 4 >= m * n * size + 4 * n
-                assert lib.gwn_linear_fwd_workspace_floats(m, n, k, elem) >= 0
+                kw = dict(M=m, N=n, K=k, elem=elem, act=2, ldw=k, ldx=k, ld_dx=k, ld_dw=k)
+                b = linear_args(_lib, _lib.LinearBwdArgs, ld_dy=n, ldz=n, **kw)
+                assert lib.gwn_linear_bwd_workspace_floats(ctypes.byref(b)) * 4 >= m * n * size + 4 * n
+                f = linear_args(_lib, _lib.LinearArgs, ldy=n, ldz=n, **{q: v for q, v in kw.items() if q[:4] != "ld_d"})
+                floats = lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f))
+                assert floats >= 0
+                f.x += size  # off a 16-byte border: x is copied
+                assert m == 0 or lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f)) * 4 >= m * k * size
 
 
 def test_modules_hold_their_parameters():
