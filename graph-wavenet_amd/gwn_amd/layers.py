@@ -63,12 +63,18 @@ def _rows(t, c):
     return t, (t.stride(0) if m > 1 else c)
 
 
-def _ws(floats, device):
-    return torch.empty(floats, device=device, dtype=F32) if floats > 0 else None
+def _ws(floats, like):
+    return like.new_empty(floats, dtype=F32) if floats > 0 else None
+
+
+def _stream(t):
+    """The raw handle of the current stream of t's device (a tenth of a microsecond; a Stream object
+    built for its handle costs up to 15, as much as a small kernel's whole launch)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 class _on:
-    """The tensors' device as the current one during a call (nothing to do where it is already)."""
+    """t's device as the current one during a call (nothing to do where it is already)."""
 
     def __init__(self, t):
         self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
@@ -82,84 +88,75 @@ class _on:
             self.guard.__exit__(*exc)
 
 
+def _backward(impl):
+    """A backward that cannot be differentiated again.  The wrapper that makes it say so is only
+    needed where the backward itself is recorded (create_graph)."""
+    recorded = once_differentiable(impl)
+    return staticmethod(lambda ctx, dy: recorded(ctx, dy) if torch.is_grad_enabled() else impl(ctx, dy))
+
+
 # ---- the product with its epilogue ----------------------------------------------------------
 
 def _linear_fwd(x, weight, bias, act, residual, p, seed, salt, keep_z):
     n, k = weight.shape
-    y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape[:-1] + (n,))
     m = y.numel() // n
     z = None
     if keep_z and act:
-        z = torch.empty(m, n, device=x.device, dtype=F32 if x.dtype == F32 else torch.float16)
+        z = x.new_empty((m, n), dtype=F32 if x.dtype == F32 else torch.float16)
     if m == 0:
         return y, z
     x, ldx = _rows(x, k)
-    w, ldw = _rows(weight, k)
-    a = _lib.LinearArgs()
-    a.x, a.ldx, a.w, a.ldw = x.data_ptr(), ldx, w.data_ptr(), ldw
-    if bias is not None:
-        bias = bias.contiguous()
-        a.bias = bias.data_ptr()
-    if residual is not None:
-        residual, a.ld_res = _rows(residual, n)
-        a.residual = residual.data_ptr()
-    a.y, a.ldy = y.data_ptr(), n
-    if z is not None:
-        a.z, a.ldz = z.data_ptr(), n
-    a.M, a.N, a.K, a.elem, a.act = m, n, k, _ELEM[x.dtype], act
-    if p > 0.0:
-        a.seed_ptr, a.salt, a.drop_p = seed.data_ptr(), salt, p
+    weight, ldw = _rows(weight, k)
+    bias = bias if bias is None else bias.contiguous()
+    residual, ldr = (None, 0) if residual is None else _rows(residual, n)
+    ptr = _lib.ptr
+    a = _lib.LinearArgs(x.data_ptr(), ldx, weight.data_ptr(), ldw, ptr(bias), ptr(residual), ldr, y.data_ptr(), n, ptr(z), n,
+                        m, n, k, _ELEM[x.dtype], act, seed.data_ptr() if p > 0.0 else None, salt, p, None)
+    at = ctypes.byref(a)
     with _on(x):
-        ws = _ws(_lib.load().gwn_linear_fwd_workspace_floats(ctypes.byref(a)), x.device)
-        a.workspace = _lib.ptr(ws)
-        _lib.call("gwn_linear_fwd", ctypes.byref(a), _lib.stream())
+        ws = _ws(_lib.load().gwn_linear_fwd_workspace_floats(at), x)
+        a.workspace = ptr(ws)
+        _lib.call("gwn_linear_fwd", at, _stream(x))
     return y, z
+
+
+def _linear_bwd(ctx, dy):
+    x, weight, z, seed = ctx.saved_tensors
+    n, k = ctx.wshape
+    needs = ctx.needs_input_grad
+    dres = dy if needs[3] else None
+    if not (needs[0] or needs[1] or needs[2]):
+        return None, None, None, dres, None, None, None, None
+    dx = dy.new_empty(ctx.shape) if needs[0] else None
+    dw = dy.new_empty((n, k)) if needs[1] else None
+    db = dy.new_empty(n) if needs[2] else None
+    m = dy.numel() // n
+    dy, ldy = _rows(dy, n)
+    x, ldx = (None, 0) if x is None else _rows(x, k)
+    weight, ldw = (None, 0) if weight is None else _rows(weight, k)
+    ptr = _lib.ptr
+    a = _lib.LinearBwdArgs(dy.data_ptr(), ldy, ptr(x), ldx, ptr(weight), ldw, ptr(z), n, ptr(dx), k, ptr(dw), k, ptr(db), m,
+                           n, k, _ELEM[dy.dtype], ctx.act, ptr(seed), ctx.salt, ctx.p, None)
+    at = ctypes.byref(a)
+    with _on(dy):
+        ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(at), dy)
+        a.workspace = ptr(ws)
+        _lib.call("gwn_linear_bwd", at, _stream(dy))
+    return dx, dw, db, dres, None, None, None, None
 
 
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, p, seed, salt):
-        needs = ctx.needs_input_grad[:3]
-        y, z = _linear_fwd(x, weight, bias, act, residual, p, seed, salt, any(needs))
+        needs = ctx.needs_input_grad
+        y, z = _linear_fwd(x, weight, bias, act, residual, p, seed, salt, needs[0] or needs[1] or needs[2])
         ctx.save_for_backward(x if needs[1] else None, weight if needs[0] else None, z, seed if p > 0.0 else None)
         ctx.shape, ctx.wshape = x.shape, weight.shape
         ctx.act, ctx.p, ctx.salt = act, p, salt
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, z, seed = ctx.saved_tensors
-        n, k = ctx.wshape
-        dev, dt = dy.device, dy.dtype
-        needs = ctx.needs_input_grad
-        dres = dy if needs[3] else None
-        dx = torch.empty(ctx.shape, device=dev, dtype=dt) if needs[0] else None
-        dw = torch.empty(n, k, device=dev, dtype=dt) if needs[1] else None
-        db = torch.empty(n, device=dev, dtype=dt) if needs[2] else None
-        if not any(needs[:3]):
-            return None, None, None, dres, None, None, None, None
-        m = dy.numel() // n
-        dy2, ld = _rows(dy, n)
-        a = _lib.LinearBwdArgs()
-        a.dy, a.ld_dy = dy2.data_ptr(), ld
-        if x is not None:
-            x, a.ldx = _rows(x, k)
-            a.x = x.data_ptr()
-        if weight is not None:
-            weight, a.ldw = _rows(weight, k)
-            a.w = weight.data_ptr()
-        if z is not None:
-            a.z, a.ldz = z.data_ptr(), n
-        a.dx, a.ld_dx, a.dw, a.ld_dw, a.dbias = _lib.ptr(dx), k, _lib.ptr(dw), k, _lib.ptr(db)
-        a.M, a.N, a.K, a.elem, a.act = m, n, k, _ELEM[dt], ctx.act
-        if seed is not None:
-            a.seed_ptr, a.salt, a.drop_p = seed.data_ptr(), ctx.salt, ctx.p
-        with _on(dy):
-            ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(ctypes.byref(a)), dev)
-            a.workspace = _lib.ptr(ws)
-            _lib.call("gwn_linear_bwd", ctypes.byref(a), _lib.stream())
-        return dx, dw, db, dres, None, None, None, None
+    backward = _backward(_linear_bwd)
 
 
 def linear_act(x, weight, bias=None, act="none", residual=None, p=0.0, seed=None, salt=0):
@@ -192,9 +189,9 @@ def linear_act(x, weight, bias=None, act="none", residual=None, p=0.0, seed=None
 
 def _norm_fwd(x, weight, bias, eps, keep):
     c = x.shape[-1]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     m = x.numel() // c
-    stats = torch.empty(2, m, device=x.device, dtype=F32) if keep else None
+    stats = x.new_empty((2, m), dtype=F32) if keep else None
     if m == 0:
         return y, stats
     x, ldx = _rows(x, c)
@@ -202,11 +199,35 @@ def _norm_fwd(x, weight, bias, eps, keep):
     bias = bias.contiguous() if bias is not None else None
     params = weight if weight is not None else bias
     wide = int(params is not None and params.dtype == F32)
+    mean = stats.data_ptr() if keep else None
     with _on(x):
-        mean = stats.data_ptr() if keep else None
         _lib.call("gwn_layernorm_fwd", x.data_ptr(), ldx, m, c, _ELEM[x.dtype], _lib.ptr(weight), _lib.ptr(bias),
-                  wide, eps, y.data_ptr(), c, mean, mean + 4 * m if keep else None, _lib.stream())
+                  wide, eps, y.data_ptr(), c, mean, mean + 4 * m if keep else None, _stream(x))
     return y, stats
+
+
+def _norm_bwd(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    c = x.shape[-1]
+    m = x.numel() // c
+    needs = ctx.needs_input_grad
+    pt = ctx.params_dtype
+    dx = x.new_empty(x.shape) if needs[0] else None
+    dw = x.new_empty(c, dtype=pt) if needs[1] else None
+    db = x.new_empty(c, dtype=pt) if needs[2] else None
+    x, ldx = _rows(x, c)
+    dy, ldy = _rows(dy, c)
+    weight = weight.contiguous() if weight is not None else None
+    elem = _ELEM[x.dtype]
+    mean = stats.data_ptr()
+    with _on(x):
+        ws = None
+        if dw is not None or db is not None:
+            ws = _ws(_lib.load().gwn_layernorm_bwd_workspace_floats(m, c, elem), x)
+        _lib.call("gwn_layernorm_bwd", dy.data_ptr(), ldy, x.data_ptr(), ldx, m, c, elem, _lib.ptr(weight),
+                  int(pt == F32), mean, mean + 4 * m, _lib.ptr(dx), c, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws),
+                  _stream(x))
+    return dx, dw, db, None
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -214,33 +235,11 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         y, stats = _norm_fwd(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        params = weight if weight is not None else bias
+        ctx.params_dtype = None if params is None else params.dtype
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        c = x.shape[-1]
-        m = x.numel() // c
-        needs = ctx.needs_input_grad
-        pt = weight.dtype if weight is not None else ctx.bias_dtype
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if needs[0] else None
-        dw = torch.empty(c, device=x.device, dtype=pt) if needs[1] else None
-        db = torch.empty(c, device=x.device, dtype=pt) if needs[2] else None
-        x2, ldx = _rows(x, c)
-        dy2, ldy = _rows(dy, c)
-        weight = weight.contiguous() if weight is not None else None
-        elem = _ELEM[x.dtype]
-        with _on(x):
-            ws = None
-            if dw is not None or db is not None:
-                ws = _ws(_lib.load().gwn_layernorm_bwd_workspace_floats(m, c, elem), x.device)
-            mean = stats.data_ptr()
-            _lib.call("gwn_layernorm_bwd", dy2.data_ptr(), ldy, x2.data_ptr(), ldx, m, c, elem, _lib.ptr(weight),
-                      int(pt == F32), mean, mean + 4 * m, _lib.ptr(dx), c, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws),
-                      _lib.stream())
-        return dx, dw, db, None
+    backward = _backward(_norm_bwd)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -268,13 +267,19 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 # ---- dropout --------------------------------------------------------------------------------
 
 def _drop(x, residual, p, seed, salt):
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None
     with _on(x):
         _lib.call("gwn_dropout", x.data_ptr(), _lib.ptr(residual), y.data_ptr(), y.numel(), _ELEM[x.dtype],
-                  seed.data_ptr(), salt, p, _lib.stream())
+                  seed.data_ptr(), salt, p, _stream(x))
     return y
+
+
+def _drop_bwd(ctx, dy):
+    needs = ctx.needs_input_grad
+    dx = _drop(dy, None, ctx.p, ctx.saved_tensors[0], ctx.salt) if needs[0] else None
+    return dx, (dy if needs[1] else None), None, None, None
 
 
 class _DropoutFn(torch.autograd.Function):
@@ -284,11 +289,7 @@ class _DropoutFn(torch.autograd.Function):
         ctx.p, ctx.salt = p, salt
         return _drop(x, residual, p, seed, salt)
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        dx = _drop(dy, None, ctx.p, ctx.saved_tensors[0], ctx.salt) if ctx.needs_input_grad[0] else None
-        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None
+    backward = _backward(_drop_bwd)
 
 
 def dropout(x, p, seed, salt=0, residual=None):
