@@ -124,7 +124,7 @@ __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int
 // step are staged in LDS by buffer loads that write LDS themselves, 16 bytes a lane, in two
 // buffers: a step's loads are in flight while the step before is multiplied.  LDS is written
 // linearly, so the swizzle that keeps the fragment reads off each other's banks is in the global
-// address: a K row's 16-byte piece c lies at c ^ (row & 7); an M row's (16-bit) at c ^ ((k & 3) << 2),
+// address: a K row's 16-byte piece c lies at c ^ ((row >> 1) & 7); an M row's (16-bit) at c ^ ((k & 3) << 2),
 // read by ds_read_b64_tr_b16, which hands each lane four k of its own column.  What lies outside
 // the matrices is a load past its buffer resource, which gives zeros.
 // An operand needs 16-byte aligned rows of whole 16-byte pieces; others are copied to such rows first.
@@ -145,10 +145,9 @@ struct Gemm {
 };
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x4 rsrc(const void* base, long bytes) {
+__device__ __forceinline__ u32x4 rsrc(const void* base, unsigned bytes) {
   const unsigned long long b = (unsigned long long)base;
-  return u32x4{(unsigned)b, (unsigned)(b >> 32) & 0xffffu, (unsigned)(bytes < 0x7fffff00L ? bytes : 0x7fffff00L),
-               0x00020000u};
+  return u32x4{(unsigned)b, (unsigned)(b >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 
 // 16 bytes a lane from `off` of the resource to LDS at `lds` + 16 lane.  In assembly because the
@@ -176,7 +175,7 @@ struct Stage {
     const int tid = threadIdx.x;
     const unsigned ldb = (unsigned)(o.ld * (long)sizeof(T));
     if (L == K_ROWS) {
-      const int c = (tid & 7) ^ ((tid >> 3) & 7);
+      const int c = (tid & 7) ^ ((tid >> 4) & 7);
       k = c * E;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -193,50 +192,53 @@ struct Stage {
       }
     }
   }
-  // step k0 .. of this operand into LDS at `to`; kend: the contraction's end
-  __device__ __forceinline__ void load(const Operand& o, int r0, int rows, int k0, int kend, int krows, unsigned to,
-                                       int wave) const {
-    const long ld = o.ld;
-    u32x4 rs;
-    bool ok = true;
+  // step k0 .. of this operand (kend: the contraction's end, past it all loads are zeros): its
+  // resource, then the loads one by one.  A tile's bytes fit 31 bits (MAX_LD).
+  u32x4 rs;
+  bool ok;
+  __device__ __forceinline__ void seek(const Operand& o, int r0, int rows, int k0, int kend, int krows) {
+    const unsigned ldb = (unsigned)o.ld * (unsigned)sizeof(T);
+    ok = true;
     if (L == K_ROWS) {
       const int nr = rows - r0 < R ? rows - r0 : R;
-      rs = rsrc((const T*)o.p + (long)r0 * ld + k0, ((long)(nr - 1) * ld + (kend - k0)) * (long)sizeof(T));
       ok = k0 + k < kend;
+      rs = rsrc((const T*)o.p + (long)r0 * o.ld + k0,
+                k0 < kend ? (unsigned)(nr - 1) * ldb + (unsigned)(kend - k0) * (unsigned)sizeof(T) : 0u);
     } else {
       const int left = (kend < krows ? kend : krows) - k0, nk = left < BK ? left : BK;
-      rs = rsrc((const T*)o.p + (long)k0 * ld + r0, ((long)(nk - 1) * ld + (rows - r0 + E - 1) / E * E) * (long)sizeof(T));
+      rs = rsrc((const T*)o.p + (long)k0 * o.ld + r0,
+                nk > 0 ? (unsigned)(nk - 1) * ldb + (unsigned)((rows - r0 + E - 1) / E) * 16u : 0u);
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) load_lds(rs, ok ? off[i] : OOR, to + (i * NT + wave * 64) * 16);
+  }
+  __device__ __forceinline__ void load(int i, unsigned to, int wave) const {
+    load_lds(rs, ok ? off[i] : OOR, to + (i * NT + wave * 64) * 16);
   }
 };
 
-// the fragments of one 32-row tile for 16 contraction values (16-bit)
-template <typename T, int L, int R>
-__device__ __forceinline__ s16x8 frag16(const char* s, int row0, int ks, int lane) {
-  if (L == K_ROWS) {
-    const int row = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
-    return *(const s16x8*)(s + row * 128 + ((c ^ (row & 7)) << 4));
-  }
-  const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
-  const int col = row0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
-  const char* at = s + k * (R * 2) + (((col >> 3) ^ ((k & 3) << 2)) << 4) + (col & 7) * 2;
-  typedef __attribute__((address_space(3))) s16x4* tr_ptr;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 4 * R * 2));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// Fragments.  16-bit: the 16 contraction values of quarter ks of a step for one 32-row tile, 8 a
+// lane; f32: 8 values, 4 a lane (k = 4 (2 ks + lane / 32) + 0 .. 3), for 4 products of 2.
+template <typename T> struct Frag { typedef s16x8 type; };
+template <> struct Frag<float> { typedef f32x4 type; };
 
-// four contraction values of one 32-row tile: k = 4 (2 q + lane / 32) + 0 .. 3 (f32)
-template <int L, int R>
-__device__ __forceinline__ f32x4 frag32(const char* s, int row0, int q, int lane) {
-  const int row = row0 + (lane & 31), c = q * 2 + (lane >> 5);
-  if (L == K_ROWS) return *(const f32x4*)(s + row * 128 + ((c ^ (row & 7)) << 4));
-  f32x4 v;
+template <typename T, int L, int R>
+__device__ __forceinline__ typename Frag<T>::type frag(const char* s, int row0, int ks, int lane) {
+  const int row = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
+  if constexpr (L == K_ROWS) {
+    return *(const typename Frag<T>::type*)(s + row * 128 + ((c ^ ((lane >> 1) & 7)) << 4));
+  } else if constexpr (sizeof(T) == 2) {
+    const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
+    const int col = row0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+    const char* at = s + k * (R * 2) + (((col >> 3) ^ ((k & 3) << 2)) << 4) + (col & 7) * 2;
+    typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 4 * R * 2));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    f32x4 v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = *(const float*)(s + (c * 4 + e) * (R * 4) + row * 4);
-  return v;
+    for (int e = 0; e < 4; ++e) v[e] = *(const float*)(s + (c * 4 + e) * (R * 4) + row * 4);
+    return v;
+  }
 }
 
 __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, bf16) {
@@ -293,49 +295,79 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  auto issue = [&](int k0, int buf) {
-    sa.load(p.a, m0, p.M, k0, kend, p.krows, lds0 + buf * STAGE, wave);
-    sb.load(p.b, n0, p.N, k0, kend, p.krows, lds0 + buf * STAGE + BM * 128, wave);
+  constexpr int LOADS = sa.PER + sb.PER;
+  auto seek = [&](int k0) {
+    sa.seek(p.a, m0, p.M, k0, kend, p.krows);
+    sb.seek(p.b, n0, p.N, k0, kend, p.krows);
   };
-  if (kbeg < kend) issue(kbeg, 0);
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
-    // this wave's loads of the step have landed; behind the barrier every wave's have, and every wave
-    // has read the other buffer for the last time
+  auto issue = [&](int i, int buf) {
+    if (i < sa.PER)
+      sa.load(i, lds0 + buf * STAGE, wave);
+    else
+      sb.load(i - sa.PER, lds0 + buf * STAGE + BM * 128, wave);
+  };
+  typename Frag<T>::type fa[2][TM], fb[2][TN];
+  auto read = [&](int buf, int ks) {
+    const char* A = smem + buf * STAGE;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[ks & 1][i] = frag<T, LA, BM>(A, wm * WTM + i * 32, ks, lane);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[ks & 1][j] = frag<T, LB, BN>(A + BM * 128, wn * WTN + j * 32, ks, lane);
+  };
+  // A quarter's products; from `first` on (-1: none) half of the loads of the step that `seek` has set
+  // go between them: all at once they would keep the wave from its products until the address unit
+  // has taken the whole workgroup's, 16 cycles each.
+  constexpr int MM = TM * TN * (sizeof(T) == 2 ? 1 : 4), EVERY = MM * 2 / LOADS > 0 ? MM * 2 / LOADS : 1;
+  auto multiply = [&](int ks, int first, int buf) {
+#pragma unroll
+    for (int q = 0; q < MM; ++q) {
+      const int e = q / (TM * TN), i = q % (TM * TN) / TN, j = q % TN;
+      if constexpr (sizeof(T) == 2)
+        acc[i][j] = mma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], T());
+      else
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[ks & 1][i][e], fb[ks & 1][j][e], acc[i][j], 0, 0, 0);
+      if ((q + 1) % EVERY == 0 && first >= 0) {
+        __builtin_amdgcn_sched_barrier(0);
+        issue(first + q / EVERY, buf);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // A step's last quarter is multiplied behind the next step's barrier: by then all its fragments are
+  // in registers, so the buffer is free for the loads of the step after next, and the next step's
+  // first fragments arrive under those products.
+  auto turn = [&]() {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (k0 + BK < kend) issue(k0 + BK, buf ^ 1);
-    const char* A = smem + buf * STAGE;
-    const char* B = A + BM * 128;
+  };
+  if (kbeg < kend) {
+    seek(kbeg);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      if constexpr (sizeof(T) == 2) {
-        s16x8 fa[TM], fb[TN];
+    for (int i = 0; i < LOADS; ++i) issue(i, 0);
+    turn();
+    seek(kbeg + BK);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) fa[i] = frag16<T, LA, BM>(A, wm * WTM + i * 32, ks, lane);
+    for (int i = 0; i < LOADS / 2; ++i) issue(i, 1);
+    read(0, 0);
+    int buf = 0;
+    for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) fb[j] = frag16<T, LB, BN>(B, wn * WTN + j * 32, ks, lane);
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = mma(fa[i], fb[j], acc[i][j], T());
-      } else {
-        f32x4 fa[TM], fb[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) fa[i] = frag32<LA, BM>(A, wm * WTM + i * 32, ks, lane);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) fb[j] = frag32<LB, BN>(B, wn * WTN + j * 32, ks, lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i][e], fb[j][e], acc[i][j], 0, 0, 0);
+      for (int ks = 0; ks < 3; ++ks) {
+        read(buf, ks + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(ks, ks == 0 ? LOADS / 2 : -1, buf ^ 1);  // the second half of the next step's loads
+        __builtin_amdgcn_sched_barrier(0);
       }
+      turn();
+      read(buf ^ 1, 0);  // past the last step: zeros, not used
+      seek(k0 + 2 * BK);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(3, 0, buf);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // the loads past the end write LDS too: vmcnt(0)
   }
 
   // 32 rows of a wave at a time through LDS, from the accumulators' layout to whole row pieces
