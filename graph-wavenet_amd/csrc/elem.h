@@ -78,53 +78,67 @@ struct DropKey {
 
 // ---- activations -----------------------------------------------------------------------------
 // FAST (16-bit results): exp and reciprocal by the hardware's instructions, erf by Abramowitz and
-// Stegun 7.1.26 (absolute error 1.5e-7, a hundredth of half a step of f16 at 1).
-template <bool FAST> __device__ __forceinline__ float exp_(float x) { return FAST ? __expf(x) : expf(x); }
+// Stegun 7.1.26 (absolute error 1.5e-7, a hundredth of half a step of f16 at 1).  Products that can meet
+// an infinity and a zero take the multiply that gives zero there, so that every activation and slope
+// has its limits at both ends, without a branch; a NaN stays one.
+template <bool FAST> __device__ __forceinline__ float exp_(float x) {
+  return FAST ? __builtin_amdgcn_exp2f(1.44269504f * x) : expf(x);
+}
 template <bool FAST> __device__ __forceinline__ float rcp_(float x) {
   return FAST ? __builtin_amdgcn_rcpf(x) : 1.0f / x;
 }
+// The instruction v_mul_legacy_f32, by the compiler's intrinsic (it has no builtin): the compiler places
+// the wait that a use of an exp or rcp result needs.
+extern "C" __device__ float gwn_fmul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float mul0(float a, float b) { return gwn_fmul_legacy(a, b); }
 
 // the normal distribution's Phi(z); e = exp(-z^2 / 2)
 template <bool FAST> __device__ __forceinline__ float normal_cdf(float z, float e) {
   if (!FAST) return 0.5f * erfcf(-0.70710678f * z);
-  const float t = rcp_<true>(1.0f + 0.3275911f * 0.70710678f * fabsf(z));
+  const float t = rcp_<true>(1.0f + 0.231641888f * fabsf(z));
   const float p =
-      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float tail = 0.5f * p * e;
+      t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+  const float tail = p * e;
   return z < 0.0f ? tail : 1.0f - tail;
 }
+// 2 sqrt(2/pi) (z + 0.044715 z^3): gelu_tanh is z / (1 + exp(-u))
+__device__ __forceinline__ float gelu_u(float z) { return z * (1.5957691216f + 0.0713548163f * z * z); }
 
-template <bool FAST> __device__ __forceinline__ float act_value(float z, int act) {
-  switch (act) {
-    case GWN_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
-    case GWN_ACT_GELU: return z * normal_cdf<FAST>(z, FAST ? exp_<FAST>(-0.5f * z * z) : 0.0f);
-    case GWN_ACT_GELU_TANH: {
-      const float u = z * (1.5957691216f + 0.0713548163f * z * z);  // 2 sqrt(2/pi) (z + 0.044715 z^3)
-      return z * rcp_<FAST>(1.0f + exp_<FAST>(-u));
-    }
-    case GWN_ACT_SILU: return z * rcp_<FAST>(1.0f + exp_<FAST>(-z));
-    default: return z;
-  }
+template <bool FAST, int ACT> __device__ __forceinline__ float act_value(float z) {
+  if (ACT == GWN_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  if (ACT == GWN_ACT_GELU) return mul0(z, normal_cdf<FAST>(z, FAST ? exp_<FAST>(-0.5f * z * z) : 0.0f));
+  if (ACT == GWN_ACT_GELU_TANH) return mul0(z, rcp_<FAST>(1.0f + exp_<FAST>(-gelu_u(z))));
+  if (ACT == GWN_ACT_SILU) return mul0(z, rcp_<FAST>(1.0f + exp_<FAST>(-z)));
+  return z;
 }
 
-// the derivative; past |z| = 50 every one of them is 0 or 1 to the last bit, and the formulas'
-// products of an infinity and a zero are not formed
-template <bool FAST> __device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == GWN_ACT_NONE) return 1.0f;
-  if (act == GWN_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (z > 50.0f) return 1.0f;
-  if (z < -50.0f) return 0.0f;
-  if (act == GWN_ACT_GELU) {
+template <bool FAST, int ACT> __device__ __forceinline__ float act_slope(float z) {
+  if (ACT == GWN_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (ACT == GWN_ACT_GELU) {
     const float e = exp_<FAST>(-0.5f * z * z);
-    return normal_cdf<FAST>(z, e) + 0.3989422804f * z * e;
+    return normal_cdf<FAST>(z, e) + mul0(0.3989422804f * z, e);
   }
-  if (act == GWN_ACT_GELU_TANH) {
-    const float z2 = z * z, u = z * (1.5957691216f + 0.0713548163f * z2);
-    const float s = rcp_<FAST>(1.0f + exp_<FAST>(-u));
-    return s + z * s * (1.0f - s) * (1.5957691216f + 0.2140644488f * z2);
+  if (ACT == GWN_ACT_GELU_TANH) {
+    const float s = rcp_<FAST>(1.0f + exp_<FAST>(-gelu_u(z)));
+    return s + mul0(s * (1.0f - s), z * (1.5957691216f + 0.2140644488f * z * z));
   }
-  const float s = rcp_<FAST>(1.0f + exp_<FAST>(-z));
-  return s * (1.0f + z * (1.0f - s));
+  if (ACT == GWN_ACT_SILU) {
+    const float s = rcp_<FAST>(1.0f + exp_<FAST>(-z));
+    return mul0(s, 1.0f + mul0(z, 1.0f - s));
+  }
+  return 1.0f;
+}
+
+// v[j] = act(v[j]), the choice made once for the V
+template <bool FAST, int ACT, int V> __device__ __forceinline__ void act_all(float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = act_value<FAST, ACT>(v[j]);
+}
+template <bool FAST, int V> __device__ __forceinline__ void act_vec(float (&v)[V], int act) {
+  if (act == GWN_ACT_RELU) act_all<FAST, GWN_ACT_RELU, V>(v);
+  if (act == GWN_ACT_GELU) act_all<FAST, GWN_ACT_GELU, V>(v);
+  if (act == GWN_ACT_GELU_TANH) act_all<FAST, GWN_ACT_GELU_TANH, V>(v);
+  if (act == GWN_ACT_SILU) act_all<FAST, GWN_ACT_SILU, V>(v);
 }
 
 template <typename T> constexpr bool is16 = sizeof(T) == 2;

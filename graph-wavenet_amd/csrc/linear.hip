@@ -25,13 +25,12 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 template <typename T> struct ZType { typedef f16 type; };
 template <> struct ZType<float> { typedef float type; };
 
-__device__ __forceinline__ float z_of(float z, float) { return z; }
-__device__ __forceinline__ f16 z_of(float z, f16) {
-  // finite values stay finite, and a positive one positive: the derivatives' limits and relu's
-  // border then come out of the rounded value as out of the exact one
-  f16 h = (f16)(fabsf(z) < 3.0e38f ? fminf(fmaxf(z, -65504.0f), 65504.0f) : z);
-  if (z > 0.0f && h == (f16)0.0f) h = (f16)5.9604645e-8f;
-  return h;
+// Past f16's range it is an infinity, where the derivatives have their limits; relu's border comes out
+// of the rounded value as out of the exact one if a positive value stays positive.
+__device__ __forceinline__ float z_of(float z, int, float) { return z; }
+__device__ __forceinline__ f16 z_of(float z, int act, f16) {
+  const f16 h = (f16)z;
+  return act == GWN_ACT_RELU && z > 0.0f && h == (f16)0.0f ? (f16)5.9604645e-8f : h;
 }
 
 struct Epi {
@@ -94,7 +93,7 @@ __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int
     Z* z = (Z*)e.z + m * e.ldz + n;
     Pack<Z, V> a;
 #pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = z_of(v[j], Z());
+    for (int j = 0; j < V; ++j) a.v[j] = z_of(v[j], e.act, Z());
     if (rem >= V) {
       store<Z, V>(z, a);
     } else {
@@ -103,10 +102,7 @@ __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int
         if (j < rem) z[j] = a.v[j];
     }
   }
-  if (e.act != GWN_ACT_NONE) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = act_value<is16<T>>(v[j], e.act);
-  }
+  act_vec<is16<T>, V>(v, e.act);
   if (e.drop.thr) drop_vec<V>(v, key, e.drop, (unsigned long long)m * e.N + n);
   if (e.res) {
     float r[V];
@@ -124,8 +120,8 @@ __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int
 // step are staged in LDS by buffer loads that write LDS themselves, 16 bytes a lane, in two
 // buffers: a step's loads are in flight while the step before is multiplied.  LDS is written
 // linearly, so the swizzle that keeps the fragment reads off each other's banks is in the global
-// address: a K row's 16-byte piece c lies at c ^ ((row >> 1) & 7); an M row's (16-bit) at c ^ ((k & 3) << 2),
-// read by ds_read_b64_tr_b16, which hands each lane four k of its own column.  What lies outside
+// address (swizzle, swizzle_m).  M rows of 16-bit values are read by ds_read_b64_tr_b16, which hands each
+// lane four k of its own column.  What lies outside
 // the matrices is a load past its buffer resource, which gives zeros.
 // An operand needs 16-byte aligned rows of whole 16-byte pieces; others are copied to such rows first.
 
@@ -163,23 +159,32 @@ __device__ __forceinline__ void load_lds(u32x4 rs, unsigned off, unsigned lds) {
       : "memory");  // m0 is reserved: the compiler sets it before each use of its own, and has none here
 }
 
-// R rows (or columns) of an operand, one step of 128 bytes of k, by NT threads
-template <typename T, int L, int R, int NT>
+// where in a K row of P pieces piece 0 lies: rows that one LDS cycle reads together (16 of them, 256
+// bytes; lanes 0-3, 12-15, 20-27 and the rest) fall on different banks
+template <int P> __device__ __forceinline__ int swizzle(int row) { return P == 8 ? (row >> 1) & 7 : (row >> 2) & 3; }
+
+// the same for an M row of 16-bit values, read 4 rows x 32 columns at a time
+template <typename T, int R> __device__ __forceinline__ int swizzle_m(int k) {
+  return sizeof(T) == 4 ? 0 : R >= 128 ? (k & 3) << 2 : R == 64 ? (k & 2) << 1 : 0;
+}
+
+// R rows (or columns) of an operand, one step of BB bytes of k, by NT threads
+template <typename T, int L, int R, int NT, int BB>
 struct Stage {
-  static constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
-  static constexpr int PER = R * 8 / NT, CPR = R * (int)sizeof(T) / 16;
-  static_assert(R * 8 % NT == 0, "whole loads");
+  static constexpr int E = 16 / (int)sizeof(T), BK = BB / (int)sizeof(T), P = BB / 16;
+  static constexpr int PER = R * P / NT, CPR = R * (int)sizeof(T) / 16;
+  static_assert(R * P % NT == 0 && NT / P % 16 == 0, "whole loads");
   unsigned off[PER];
   int k;  // K rows: this thread's k within a step
   __device__ __forceinline__ void init(const Operand& o, int r0, int rows) {
     const int tid = threadIdx.x;
     const unsigned ldb = (unsigned)(o.ld * (long)sizeof(T));
     if (L == K_ROWS) {
-      const int c = (tid & 7) ^ ((tid >> 4) & 7);
+      const int c = (tid % P) ^ swizzle<P>(tid / P);
       k = c * E;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int r = i * (NT / 8) + (tid >> 3);
+        const int r = i * (NT / P) + tid / P;
         off[i] = r0 + r < rows ? r * ldb + c * 16 : OOR;
       }
     } else {
@@ -187,7 +192,7 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int q = i * NT + tid, kk = q / CPR;
-        const int c = (q % CPR) ^ (sizeof(T) == 2 ? (kk & 3) << 2 : 0);
+        const int c = (q % CPR) ^ swizzle_m<T, R>(kk);
         off[i] = r0 + c * E < rows ? kk * ldb + c * 16 : OOR;
       }
     }
@@ -220,15 +225,15 @@ struct Stage {
 template <typename T> struct Frag { typedef s16x8 type; };
 template <> struct Frag<float> { typedef f32x4 type; };
 
-template <typename T, int L, int R>
+template <typename T, int L, int R, int BB>
 __device__ __forceinline__ typename Frag<T>::type frag(const char* s, int row0, int ks, int lane) {
   const int row = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
   if constexpr (L == K_ROWS) {
-    return *(const typename Frag<T>::type*)(s + row * 128 + ((c ^ ((lane >> 1) & 7)) << 4));
+    return *(const typename Frag<T>::type*)(s + row * BB + ((c ^ swizzle<BB / 16>(lane & 31)) << 4));
   } else if constexpr (sizeof(T) == 2) {
     const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
     const int col = row0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
-    const char* at = s + k * (R * 2) + (((col >> 3) ^ ((k & 3) << 2)) << 4) + (col & 7) * 2;
+    const char* at = s + k * (R * 2) + (((col >> 3) ^ swizzle_m<T, R>(k)) << 4) + (col & 7) * 2;
     typedef __attribute__((address_space(3))) s16x4* tr_ptr;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 4 * R * 2));
@@ -250,8 +255,8 @@ __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, f16) {
 }
 
 // workgroup -> (tile, split).  Consecutive workgroups go to the 8 XCDs in turn: each XCD gets a
-// contiguous run of tiles, 8 rows of tiles walked column by column, so that its L2 holds the operands
-// they share.
+// contiguous run of tiles, 4 rows of tiles walked column by column, so that its L2 holds the operands
+// they share (2 to 16 rows measure within 5%).
 __device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& split) {
   const int total = gridDim.x, per = total >> 3;
   int id = blockIdx.x;
@@ -259,19 +264,19 @@ __device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& spli
   const int tiles = p.tiles_m * p.tiles_n;
   split = id / tiles;
   id -= split * tiles;
-  const int width = 8 * p.tiles_n, g = id / width, first = g * 8;
-  const int rows = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
+  const int width = 4 * p.tiles_n, g = id / width, first = g * 4;
+  const int rows = p.tiles_m - first < 4 ? p.tiles_m - first : 4;
   id -= g * width;
   tn = id / rows;
   tm = first + id - tn * rows;
 }
 
-template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN>
+template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN, int BB, int S>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   constexpr int NT = 64 * WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 32, TN = WTN / 32;
-  constexpr int BK = 128 / (int)sizeof(T), STAGE = (BM + BN) * 128;
+  constexpr int BK = BB / (int)sizeof(T), Q = BB / 32, STAGE = (BM + BN) * BB;
   constexpr int EW = WTN + 4;  // floats a row of the epilogue's image of one wave's 32 rows
-  constexpr int SMEM = 2 * STAGE > WGM * WGN * 32 * EW * 4 ? 2 * STAGE : WGM * WGN * 32 * EW * 4;
+  constexpr int SMEM = S * STAGE > WGM * WGN * 32 * EW * 4 ? S * STAGE : WGM * WGN * 32 * EW * 4;
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -282,8 +287,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   const int m0 = tm * BM, n0 = tn * BN;
   const int kbeg = split * p.kchunk, kend = p.K - kbeg < p.kchunk ? p.K : kbeg + p.kchunk;
 
-  Stage<T, LA, BM, NT> sa;
-  Stage<T, LB, BN, NT> sb;
+  Stage<T, LA, BM, NT, BB> sa;
+  Stage<T, LB, BN, NT, BB> sb;
   sa.init(p.a, m0, p.M);
   sb.init(p.b, n0, p.N);
 
@@ -304,21 +309,21 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
     if (i < sa.PER)
       sa.load(i, lds0 + buf * STAGE, wave);
     else
-      sb.load(i - sa.PER, lds0 + buf * STAGE + BM * 128, wave);
+      sb.load(i - sa.PER, lds0 + buf * STAGE + BM * BB, wave);
   };
   typename Frag<T>::type fa[2][TM], fb[2][TN];
   auto read = [&](int buf, int ks) {
     const char* A = smem + buf * STAGE;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fa[ks & 1][i] = frag<T, LA, BM>(A, wm * WTM + i * 32, ks, lane);
+    for (int i = 0; i < TM; ++i) fa[ks & 1][i] = frag<T, LA, BM, BB>(A, wm * WTM + i * 32, ks, lane);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fb[ks & 1][j] = frag<T, LB, BN>(A + BM * 128, wn * WTN + j * 32, ks, lane);
+    for (int j = 0; j < TN; ++j) fb[ks & 1][j] = frag<T, LB, BN, BB>(A + BM * BB, wn * WTN + j * 32, ks, lane);
   };
-  // A quarter's products; from `first` on (-1: none) half of the loads of the step that `seek` has set
-  // go between them: all at once they would keep the wave from its products until the address unit
-  // has taken the whole workgroup's, 16 cycles each.
-  constexpr int MM = TM * TN * (sizeof(T) == 2 ? 1 : 4), EVERY = MM * 2 / LOADS > 0 ? MM * 2 / LOADS : 1;
-  auto multiply = [&](int ks, int first, int buf) {
+  // A part's products (32 bytes of k).  The step's loads go between those of its first SPREAD parts:
+  // all at once they would keep the wave from its products until the address unit has taken the
+  // whole workgroup's, 16 cycles each.
+  constexpr int MM = TM * TN * (sizeof(T) == 2 ? 1 : 4), SPREAD = S == 2 ? Q / 2 : Q;
+  auto multiply = [&](int ks, int part, int to) {
 #pragma unroll
     for (int q = 0; q < MM; ++q) {
       const int e = q / (TM * TN), i = q % (TM * TN) / TN, j = q % TN;
@@ -326,45 +331,57 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
         acc[i][j] = mma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], T());
       else
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[ks & 1][i][e], fb[ks & 1][j][e], acc[i][j], 0, 0, 0);
-      if ((q + 1) % EVERY == 0 && first >= 0) {
-        __builtin_amdgcn_sched_barrier(0);
-        issue(first + q / EVERY, buf);
-        __builtin_amdgcn_sched_barrier(0);
+      // loads l with l / LOADS < (part MM + q + 1) / (SPREAD MM)
+      if (part < SPREAD) {
+        const int done = (part * MM + q) * LOADS / (SPREAD * MM), next = (part * MM + q + 1) * LOADS / (SPREAD * MM);
+        if (next > done) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int l = done; l < next; ++l) issue(l, to);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   };
-  // A step's last quarter is multiplied behind the next step's barrier: by then all its fragments are
-  // in registers, so the buffer is free for the loads of the step after next, and the next step's
-  // first fragments arrive under those products.
+  // S buffers: while one is multiplied the next S - 1 are in flight or landed.  A step's last part is
+  // multiplied behind the barrier that ends it: by then all its fragments are in registers, so its
+  // buffer is free for the loads of the step S - 1 later, and the next step's first fragments arrive
+  // under those products.
   auto turn = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    static_assert((S - 2) * LOADS < 16, "vmcnt in one field");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (S - 2) * LOADS);  // vmcnt: all but the last S - 2 steps' loads; lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   if (kbeg < kend) {
-    seek(kbeg);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) issue(i, 0);
+    for (int b = 0; b < S - 1; ++b) {
+      seek(kbeg + b * BK);
+#pragma unroll
+      for (int l = 0; l < LOADS; ++l) issue(l, b);
+    }
     turn();
-    seek(kbeg + BK);
-#pragma unroll
-    for (int i = 0; i < LOADS / 2; ++i) issue(i, 1);
     read(0, 0);
-    int buf = 0;
-    for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
+    seek(kbeg + (S - 1) * BK);
+    int buf = 0, to = S - 1;
 #pragma unroll
-      for (int ks = 0; ks < 3; ++ks) {
+    for (int l = 0; l < LOADS / SPREAD; ++l) issue(l, to);
+    for (int k0 = kbeg; k0 < kend; k0 += BK) {
+#pragma unroll
+      for (int ks = 0; ks < Q - 1; ++ks) {
         read(buf, ks + 1);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(ks, ks == 0 ? LOADS / 2 : -1, buf ^ 1);  // the second half of the next step's loads
+        multiply(ks, ks + 1, to);
         __builtin_amdgcn_sched_barrier(0);
       }
       turn();
-      read(buf ^ 1, 0);  // past the last step: zeros, not used
-      seek(k0 + 2 * BK);
+      to = buf;
+      buf = buf + 1 == S ? 0 : buf + 1;
+      read(buf, 0);  // past the last step: zeros, not used
+      seek(k0 + S * BK);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(3, 0, buf);
+      multiply(Q - 1, 0, to);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // the loads past the end write LDS too: vmcnt(0)
@@ -405,26 +422,43 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   }
 }
 
-// the splits' sums, in their order, and the epilogue: V columns a thread
-template <typename T>
+// The splits' sums and the epilogue.  256 / TY pieces of 4 columns x TY lanes of splits a workgroup:
+// where there are few outputs their many splits are read side by side.  Fixed order: a lane's splits
+// as they come, then the lanes.
+template <typename T, int TY>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int M, int N, Epi e) {
-  constexpr int V = 4;
+  constexpr int V = 4, TX = 256 / TY;
+  __shared__ float sums[TY][TX * V];
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const long per = (N + V - 1) / V, total = per * M;
   DropKey key;
-  if (e.drop.thr) key.init(e.drop, (unsigned long long)blockIdx.x * 256 * V);
-  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
-    const long m = q / per;
-    const int n = (int)(q - m * per) * V, rem = N - n;
+  if (e.drop.thr) key.init(e.drop, (unsigned long long)blockIdx.x * TX * V);
+  for (long base = (long)blockIdx.x * TX; base < total; base += (long)gridDim.x * TX) {
+    const long q = base + tx, m = q / per;
+    const int n = (int)(q - m * per) * V, rem = q < total ? N - n : 0;
     const float* at = part + m * N + n;
     float v[V] = {};
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
+    for (int s = ty; s < splits; s += TY) {
       float o[V];
       load_f<float, V>(o, at + (long)s * M * N, rem);
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] += o[j];
     }
-    epilogue<T, V>(e, key, m, n, rem, v);
+    if (TY > 1) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) sums[ty][tx * V + j] = v[j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 0.0f;
+      if (ty == 0)
+#pragma unroll
+        for (int y = 0; y < TY; ++y)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] += sums[y][tx * V + j];
+      __syncthreads();
+    }
+    if (ty == 0 && rem > 0) epilogue<T, V>(e, key, m, n, rem, v);
   }
 }
 
@@ -455,18 +489,19 @@ struct Dz {
   const void* z; long ldz;
   void* dz; int ld;  // [M][ld], columns past N zero; NULL = not written
   float* part;       // [gridDim.y][N] column sums, NULL = not wanted
-  int M, N, act;
+  int M, N, tx;  // TX = 1 << tx
   Drop drop;
 };
 
 // TX pieces of 16 bytes of columns x 256 / TX rows a workgroup, rows split over gridDim.y; each
 // thread sums its columns in fp32 before dz is rounded.  Bound by memory: dy and z read, dz written.
-template <typename T, int TX>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
   typedef typename ZType<T>::type Z;
-  constexpr int V = Vec<T>::N, TY = 256 / TX;
-  __shared__ float cols[TY][TX * V + 1];
-  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  constexpr int V = Vec<T>::N;
+  const int TX = 1 << p.tx, TY = 256 >> p.tx;
+  __shared__ float cols[256 * V];  // [TY][TX * V]
+  const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x >> p.tx;
   const long n = ((long)blockIdx.x * TX + tx) * V;
   const int rem = (int)(p.N - n < V ? p.N - n : V);
   float sum[V] = {};
@@ -474,14 +509,13 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
   if (p.drop.thr) key.init(p.drop, (unsigned long long)blockIdx.y * TY * p.N);
   if (rem > 0)
     for (long m = (long)blockIdx.y * TY + ty; m < p.M; m += (long)gridDim.y * TY) {
-      float v[V];
+      float v[V], z[V];
       load_f<T, V>(v, (const T*)p.dy + m * p.ld_dy + n, rem);
+      if (ACT != GWN_ACT_NONE) load_f<Z, V>(z, (const Z*)p.z + m * p.ldz + n, rem);
       if (p.drop.thr) drop_vec<V>(v, key, p.drop, (unsigned long long)m * p.N + n);
-      if (p.act != GWN_ACT_NONE) {
-        float z[V];
-        load_f<Z, V>(z, (const Z*)p.z + m * p.ldz + n, rem);
+      if (ACT != GWN_ACT_NONE) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= act_slope<is16<T>>(z[j], p.act);
+        for (int j = 0; j < V; ++j) v[j] *= act_slope<is16<T>, ACT>(z[j]);
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -492,14 +526,13 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
     }
   if (!p.part) return;
 #pragma unroll
-  for (int j = 0; j < V; ++j) cols[ty][tx * V + j] = sum[j];
+  for (int j = 0; j < V; ++j) cols[threadIdx.x * V + j] = sum[j];
   __syncthreads();
   for (int k = threadIdx.x; k < TX * V; k += 256) {
     const long at = (long)blockIdx.x * TX * V + k;
     if (at < p.N) {
       float v = 0.0f;
-#pragma unroll
-      for (int q = 0; q < TY; ++q) v += cols[q][k];
+      for (int q = 0; q < TY; ++q) v += cols[q * TX * V + k];
       p.part[(long)blockIdx.y * p.N + at] = v;
     }
   }
@@ -537,64 +570,85 @@ bool stageable(const void* p, long ld, int cols, int elem) {
 // floats of a copy with whole pieces a row
 long copy_floats(long rows, int cols, int elem) { return up(rows * up(cols, vec_of(elem)) * elem_bytes(elem), 16) / 4; }
 
-struct Shape { int bm, bn, tiles_m, tiles_n, splits, kchunk; };
+// The tile and the number of splits of the contraction, by the time a model gives them (cycles):
+//   rounds of tiles on a compute unit x (steps x the slower of products and loads + a fixed part)
+//   + writing and reading the splits' sums.
+// Rates are of the tile kernel on its own (bf16 8192^3: 256 x 256 1310 TFLOP/s, 128 x 128 900), a load
+// costs a compute unit a cycle per 24 bytes.
+struct Tile { int bm, bn; float rate16, rate32; };  // share of the peak rate
+constexpr Tile TILES[] = {{256, 256, 0.72f, 0.0f}, {128, 128, 0.60f, 0.90f}, {128, 64, 0.50f, 0.88f},
+                          {64, 64, 0.40f, 0.85f},  {128, 32, 0.35f, 0.80f},  {32, 128, 0.35f, 0.80f}};
+struct Shape { int tile, tiles_m, tiles_n, splits, kchunk; };
 
 Shape shape_of(int M, int N, int K, int elem) {
-  Shape s;
-  const long cus = gwn_device_cus();
-  const bool big = elem != GWN_ELEM_F32 && ((M + 255L) / 256) * ((N + 255L) / 256) >= cus;
-  s.bm = s.bn = big ? 256 : 128;
-  s.tiles_m = (M + s.bm - 1) / s.bm;
-  s.tiles_n = (N + s.bn - 1) / s.bn;
-  const long tiles = (long)s.tiles_m * s.tiles_n;
-  const int bk = 128 / elem_bytes(elem);
-  const long steps = (K + bk - 1) / bk;
-  long splits = 1;
-  if (tiles < cus) {
-    splits = (2 * cus) / tiles;
-    if (splits > steps / 4) splits = steps / 4;
-    if (splits < 1) splits = 1;
+  const bool wide = elem == GWN_ELEM_F32;
+  const int bk = wide ? 32 : 64;
+  const long cus = gwn_device_cus(), steps = (K + bk - 1) / bk;
+  Shape best{};
+  double least = 1e300;
+  for (int t = 0; t < 6; ++t) {
+    const Tile& c = TILES[t];
+    const double rate = wide ? c.rate32 * 256.0 : c.rate16 * 4096.0;
+    if (rate == 0.0) continue;
+    const long tm = (M + c.bm - 1) / c.bm, tn = (N + c.bn - 1) / c.bn, tiles = tm * tn;
+    const double product = 2.0 * c.bm * c.bn * bk / rate, loads = (c.bm + c.bn) * 128.0 / 24.0;
+    const double step = product > loads ? product : loads;
+    long last = 0;
+    for (long want = 1; want <= 512; want += (want + 3) / 4) {
+      const long chunk = (steps + want - 1) / want, splits = chunk ? (steps + chunk - 1) / chunk : 1;
+      if (splits == last) continue;
+      last = splits;
+      const long rounds = (tiles * splits + cus - 1) / cus;
+      const double join = splits > 1 ? 8000.0 + 8.0 * M * N * splits / 2000.0 : 0.0;
+      const double time = rounds * (chunk * step + 3000.0) + join;
+      if (time < least) {
+        least = time;
+        best = {t, (int)tm, (int)tn, (int)splits, (int)(chunk * bk)};
+      }
+      if (tiles * splits > 4 * cus) break;
+    }
   }
-  s.kchunk = (int)((steps + splits - 1) / splits) * bk;
-  s.splits = K ? (K + s.kchunk - 1) / s.kchunk : 1;
-  if (s.splits < 1) s.splits = 1;
-  return s;
+  return best;
 }
 long part_floats(int M, int N, int K, int elem) {
   const Shape s = shape_of(M, N, K, elem);
   return s.splits > 1 ? up((long)s.splits * M * N, 4) : 0;
 }
 
+template <typename T, int LA, int LB>
+void launch_tiles(const Gemm& p, int tile, int grid, hipStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (tile == 0) gemm_kernel<T, LA, LB, 256, 256, 2, 4, 128, 2><<<grid, 512, 0, s>>>(p);
+  if (tile == 1) gemm_kernel<T, LA, LB, 128, 128, 2, 2, 128, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 2) gemm_kernel<T, LA, LB, 128, 64, 2, 2, 128, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 3) gemm_kernel<T, LA, LB, 64, 64, 2, 2, 128, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 4) gemm_kernel<T, LA, LB, 128, 32, 4, 1, 128, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 5) gemm_kernel<T, LA, LB, 32, 128, 1, 4, 128, 2><<<grid, 256, 0, s>>>(p);
+}
+
 template <typename T>
 int gemm(int la, int lb, Operand a, Operand b, int M, int N, int K, int krows, int elem, const Epi& e, float* part,
          hipStream_t s) {
   const Shape sh = shape_of(M, N, K, elem);
-  const long tiles = (long)sh.tiles_m * sh.tiles_n * sh.splits;
-  GWN_REQUIRE(tiles < (1L << 22), "linear: too many tiles for one launch");
-  Gemm p{a, b, M, N, K, krows, sh.tiles_m, sh.tiles_n, sh.splits, sh.kchunk, part, e};
-  const int grid = (int)tiles;
-  if constexpr (sizeof(T) == 2) {
-    if (sh.bm == 256) {
-      if (la == K_ROWS && lb == K_ROWS)
-        gemm_kernel<T, K_ROWS, K_ROWS, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
-      else if (la == K_ROWS)
-        gemm_kernel<T, K_ROWS, M_ROWS, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
-      else
-        gemm_kernel<T, M_ROWS, M_ROWS, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
-    }
-  }
-  if (sh.bm == 128) {
-    if (la == K_ROWS && lb == K_ROWS)
-      gemm_kernel<T, K_ROWS, K_ROWS, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
-    else if (la == K_ROWS)
-      gemm_kernel<T, K_ROWS, M_ROWS, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
-    else
-      gemm_kernel<T, M_ROWS, M_ROWS, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
-  }
+  const long grid = (long)sh.tiles_m * sh.tiles_n * sh.splits;
+  GWN_REQUIRE(grid < (1L << 22), "linear: too many tiles for one launch");
+  const Gemm p{a, b, M, N, K, krows, sh.tiles_m, sh.tiles_n, sh.splits, sh.kchunk, part, e};
+  if (la == K_ROWS && lb == K_ROWS)
+    launch_tiles<T, K_ROWS, K_ROWS>(p, sh.tile, (int)grid, s);
+  else if (la == K_ROWS)
+    launch_tiles<T, K_ROWS, M_ROWS>(p, sh.tile, (int)grid, s);
+  else
+    launch_tiles<T, M_ROWS, M_ROWS>(p, sh.tile, (int)grid, s);
   GWN_CHECK_LAUNCH();
   if (sh.splits > 1) {
-    const long want = ((long)M * ((N + 3) / 4) + 255) / 256, most = (long)gwn_device_cus() * 16;
-    join_kernel<T><<<(int)(want < most ? want : most), 256, 0, s>>>(part, sh.splits, M, N, e);
+    const long pieces = (long)M * ((N + 3) / 4), cus = gwn_device_cus(), most = cus * 16;
+    if (pieces >= cus * 256 || sh.splits < 8) {
+      const long want = (pieces + 255) / 256;
+      join_kernel<T, 1><<<(int)(want < most ? want : most), 256, 0, s>>>(part, sh.splits, M, N, e);
+    } else {
+      const long want = (pieces + 15) / 16;
+      join_kernel<T, 16><<<(int)(want < most ? want : most), 256, 0, s>>>(part, sh.splits, M, N, e);
+    }
     GWN_CHECK_LAUNCH();
   }
   return GWN_OK;
@@ -650,8 +704,8 @@ BwdPlan bwd_plan(const gwn_linear_bwd_args* a) {
   q.copy_w = a->dx && a->M && !stageable(a->w, a->ldw, a->K, a->elem);
   q.ld_dz = (int)up(a->N, v);
   const int pieces = q.ld_dz / v;
-  q.tx = pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : 64;
-  const long bx = (pieces + q.tx - 1) / q.tx, ty = 256 / q.tx;
+  q.tx = pieces <= 8 ? 3 : pieces <= 16 ? 4 : pieces <= 32 ? 5 : 6;
+  const long bx = (pieces + (1 << q.tx) - 1) >> q.tx, ty = 256 >> q.tx;
   long parts = (8L * gwn_device_cus() + bx - 1) / bx, most = (a->M + 4 * ty - 1) / (4 * ty);
   if (parts > most) parts = most;
   if (parts > 1024) parts = 1024;
@@ -684,12 +738,13 @@ int bwd(const gwn_linear_bwd_args* a, hipStream_t s) {
   }
   if (q.write_dz || a->dbias) {
     const Dz d{a->dy, a->ld_dy, a->z, a->ldz, q.write_dz ? (void*)dz.p : nullptr, q.ld_dz, a->dbias ? sums : nullptr, a->M,
-               a->N, a->act, drop};
-    const dim3 grid((q.ld_dz / vec_of(a->elem) + q.tx - 1) / q.tx, q.parts);
-    if (q.tx == 8) dz_kernel<T, 8><<<grid, 256, 0, s>>>(d);
-    if (q.tx == 16) dz_kernel<T, 16><<<grid, 256, 0, s>>>(d);
-    if (q.tx == 32) dz_kernel<T, 32><<<grid, 256, 0, s>>>(d);
-    if (q.tx == 64) dz_kernel<T, 64><<<grid, 256, 0, s>>>(d);
+               a->N, q.tx, drop};
+    const dim3 grid((q.ld_dz / vec_of(a->elem) + (1 << q.tx) - 1) >> q.tx, q.parts);
+    if (a->act == GWN_ACT_NONE) dz_kernel<T, GWN_ACT_NONE><<<grid, 256, 0, s>>>(d);
+    if (a->act == GWN_ACT_RELU) dz_kernel<T, GWN_ACT_RELU><<<grid, 256, 0, s>>>(d);
+    if (a->act == GWN_ACT_GELU) dz_kernel<T, GWN_ACT_GELU><<<grid, 256, 0, s>>>(d);
+    if (a->act == GWN_ACT_GELU_TANH) dz_kernel<T, GWN_ACT_GELU_TANH><<<grid, 256, 0, s>>>(d);
+    if (a->act == GWN_ACT_SILU) dz_kernel<T, GWN_ACT_SILU><<<grid, 256, 0, s>>>(d);
     GWN_CHECK_LAUNCH();
   }
   if (a->dbias) {
