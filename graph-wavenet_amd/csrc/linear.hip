@@ -489,11 +489,11 @@ struct Dz {
   const void* z; long ldz;
   void* dz; int ld;  // [M][ld], columns past N zero; NULL = not written
   float* part;       // [gridDim.y][N] column sums, NULL = not wanted
-  int M, N, tx;  // TX = 1 << tx
+  int M, N, tx, stripe;  // TX = 1 << tx; rows a workgroup
   Drop drop;
 };
 
-// TX pieces of 16 bytes of columns x 256 / TX rows a workgroup, rows split over gridDim.y; each
+// TX pieces of 16 bytes of columns x a stripe of rows a workgroup, 256 / TX rows at a time; each
 // thread sums its columns in fp32 before dz is rounded.  Bound by memory: dy and z read, dz written.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
@@ -506,23 +506,31 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
   const int rem = (int)(p.N - n < V ? p.N - n : V);
   float sum[V] = {};
   DropKey key;
-  if (p.drop.thr) key.init(p.drop, (unsigned long long)blockIdx.y * TY * p.N);
+  if (p.drop.thr) key.init(p.drop, (unsigned long long)blockIdx.y * p.stripe * p.N);
+  const long first = (long)blockIdx.y * p.stripe, last = first + p.stripe < p.M ? first + p.stripe : p.M;
   if (rem > 0)
-    for (long m = (long)blockIdx.y * TY + ty; m < p.M; m += (long)gridDim.y * TY) {
-      float v[V], z[V];
-      load_f<T, V>(v, (const T*)p.dy + m * p.ld_dy + n, rem);
-      if (ACT != GWN_ACT_NONE) load_f<Z, V>(z, (const Z*)p.z + m * p.ldz + n, rem);
-      if (p.drop.thr) drop_vec<V>(v, key, p.drop, (unsigned long long)m * p.N + n);
-      if (ACT != GWN_ACT_NONE) {
+    for (long m = first + ty; m < last; m += 2 * TY) {  // two rows: their loads are in flight together
+      float v[2][V], z[2][V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= act_slope<is16<T>, ACT>(z[j]);
+      for (int u = 0; u < 2; ++u) {
+        const long r = m + u * TY;
+        const int here = r < last ? rem : 0;
+        load_f<T, V>(v[u], (const T*)p.dy + r * p.ld_dy + n, here);
+        if (ACT != GWN_ACT_NONE) load_f<Z, V>(z[u], (const Z*)p.z + r * p.ldz + n, here);
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j >= rem) v[j] = 0.0f;
-        sum[j] += v[j];
+      for (int u = 0; u < 2; ++u) {
+        const long r = m + u * TY;
+        if (r >= last) break;
+        if (p.drop.thr) drop_vec<V>(v[u], key, p.drop, (unsigned long long)r * p.N + n);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (ACT != GWN_ACT_NONE) v[u][j] *= act_slope<is16<T>, ACT>(z[u][j]);
+          if (j >= rem) v[u][j] = 0.0f;
+          sum[j] += v[u][j];
+        }
+        if (p.dz) store_f<T, V>((T*)p.dz + r * p.ld + n, v[u], V);
       }
-      if (p.dz) store_f<T, V>((T*)p.dz + m * p.ld + n, v, V);
     }
   if (!p.part) return;
 #pragma unroll
@@ -576,8 +584,8 @@ long copy_floats(long rows, int cols, int elem) { return up(rows * up(cols, vec_
 // Rates are of the tile kernel on its own (bf16 8192^3: 256 x 256 1310 TFLOP/s, 128 x 128 900), a load
 // costs a compute unit a cycle per 24 bytes.
 struct Tile { int bm, bn; float rate16, rate32; };  // share of the peak rate
-constexpr Tile TILES[] = {{256, 256, 0.72f, 0.0f}, {128, 128, 0.60f, 0.90f}, {128, 64, 0.50f, 0.88f},
-                          {64, 64, 0.40f, 0.85f},  {128, 32, 0.35f, 0.80f},  {32, 128, 0.35f, 0.80f}};
+constexpr Tile TILES[] = {{256, 256, 0.72f, 0.0f}, {128, 128, 0.60f, 0.80f}, {128, 64, 0.50f, 0.86f},
+                          {64, 64, 0.40f, 0.90f},  {128, 32, 0.35f, 0.88f},  {32, 128, 0.35f, 0.86f}};
 struct Shape { int tile, tiles_m, tiles_n, splits, kchunk; };
 
 Shape shape_of(int M, int N, int K, int elem) {
@@ -600,7 +608,7 @@ Shape shape_of(int M, int N, int K, int elem) {
       last = splits;
       const long rounds = (tiles * splits + cus - 1) / cus;
       const double join = splits > 1 ? 8000.0 + 8.0 * M * N * splits / 2000.0 : 0.0;
-      const double time = rounds * (chunk * step + 3000.0) + join;
+      const double time = rounds * (chunk * step + 2000.0 + c.bm * c.bn / 6.0) + join;
       if (time < least) {
         least = time;
         best = {t, (int)tm, (int)tn, (int)splits, (int)(chunk * bk)};
@@ -692,7 +700,7 @@ int fwd(const gwn_linear_args* a, hipStream_t s) {
 
 struct BwdPlan {
   bool write_dz, copy_x, copy_w;  // dz apart from dy; operands that have to be copied
-  int parts, tx, ld_dz;
+  int parts, tx, stripe, ld_dz;
   long floats;
 };
 BwdPlan bwd_plan(const gwn_linear_bwd_args* a) {
@@ -709,7 +717,9 @@ BwdPlan bwd_plan(const gwn_linear_bwd_args* a) {
   long parts = (8L * gwn_device_cus() + bx - 1) / bx, most = (a->M + 4 * ty - 1) / (4 * ty);
   if (parts > most) parts = most;
   if (parts > 1024) parts = 1024;
-  q.parts = (int)(parts < 1 ? 1 : parts);
+  if (parts < 1) parts = 1;
+  q.stripe = (int)up((a->M + parts - 1) / parts, 2 * ty);
+  q.parts = a->M ? (a->M + q.stripe - 1) / q.stripe : 1;
   q.floats = a->dbias ? up((long)q.parts * a->N, 4) : 0;
   if (q.write_dz) q.floats += copy_floats(a->M, a->N, a->elem);
   if (q.copy_x) q.floats += copy_floats(a->M, a->K, a->elem);
@@ -738,7 +748,7 @@ int bwd(const gwn_linear_bwd_args* a, hipStream_t s) {
   }
   if (q.write_dz || a->dbias) {
     const Dz d{a->dy, a->ld_dy, a->z, a->ldz, q.write_dz ? (void*)dz.p : nullptr, q.ld_dz, a->dbias ? sums : nullptr, a->M,
-               a->N, q.tx, drop};
+               a->N, q.tx, q.stripe, drop};
     const dim3 grid((q.ld_dz / vec_of(a->elem) + (1 << q.tx) - 1) >> q.tx, q.parts);
     if (a->act == GWN_ACT_NONE) dz_kernel<T, GWN_ACT_NONE><<<grid, 256, 0, s>>>(d);
     if (a->act == GWN_ACT_RELU) dz_kernel<T, GWN_ACT_RELU><<<grid, 256, 0, s>>>(d);
