@@ -462,6 +462,86 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   }
 }
 
+// ---- few rows -------------------------------------------------------------------------------------
+//
+// y for at most 16 MT rows of x: bound by reading w once, so w goes from memory straight into
+// v_mfma_f32_16x16x32 (16-bit) or 16x16x4 fragments.  A workgroup has 16 columns (w rows), its waves
+// split the contraction: 4 loads of 16 bytes a lane, 256 bytes of each w row, are in flight a wave and
+// turn, x's pieces come from the caches.  The waves' sums meet in LDS, then the epilogue.  Rows may
+// start anywhere; a piece over the contraction's end is loaded by element.
+struct Few {
+  const void* x; long ldx;
+  const void* w; long ldw;
+  int M, N, K;
+  Epi e;
+};
+
+__device__ __forceinline__ f32x4 mma16(Pack<bf16, 8> a, Pack<bf16, 8> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(Pack<f16, 8> a, Pack<f16, 8> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(Pack<float, 4> a, Pack<float, 4> b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
+  return c;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_part(const T* p, int rem) {
+  if (rem >= V) return load<T, V>(p);
+  Pack<T, V> a;
+#pragma unroll
+  for (int j = 0; j < V; ++j) a.v[j] = j < rem ? p[j] : (T)0.0f;
+  return a;
+}
+
+template <typename T, int MT>
+__global__ __launch_bounds__(1024) void few_kernel(const Few p) {
+  constexpr int V = Vec<T>::N, KS = 4 * V, U = 4, LD = 20;
+  __shared__ __attribute__((aligned(16))) float sums[16][16 * MT][LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int n0 = blockIdx.x * 16, row = lane & 15, kl = (lane >> 4) * V;
+  const T* w = (const T*)p.w + (long)(n0 + row < p.N ? n0 + row : p.N - 1) * p.ldw;
+  const T* x[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) x[i] = (const T*)p.x + (long)(i * 16 + row < p.M ? i * 16 + row : p.M - 1) * p.ldx;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = wave * KS * U; k0 < p.K; k0 += waves * KS * U) {
+    Pack<T, V> a[U], b[MT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * KS + kl;
+      a[u] = load_part<T, V>(w + k, p.K - k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) b[i][u] = load_part<T, V>(x[i] + k, p.K - k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = mma16(b[i][u], a[u], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sums[wave][i * 16 + (lane >> 4) * 4 + r][row] = acc[i][r];
+  __syncthreads();
+  DropKey key;
+  if (p.e.drop.thr) key.init(p.e.drop, (unsigned long long)n0);
+  for (int q = threadIdx.x; q < 16 * MT * 4; q += blockDim.x) {
+    const int m = q >> 2, n = n0 + (q & 3) * 4, rem = p.N - n;
+    if (m < p.M && rem > 0) {
+      float v[4] = {};
+      for (int s = 0; s < waves; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += sums[s][m][(q & 3) * 4 + j];
+      epilogue<T, 4>(p.e, key, m, n, rem, v);
+    }
+  }
+}
+
 // rows [rows][ld] -> [rows][ldo] with zeros past `cols`: a 16-byte piece a thread
 template <typename T>
 __global__ __launch_bounds__(256) void copy_rows_kernel(const T* x, long ld, long rows, int cols, T* o, int ldo) {
@@ -578,37 +658,45 @@ bool stageable(const void* p, long ld, int cols, int elem) {
 // floats of a copy with whole pieces a row
 long copy_floats(long rows, int cols, int elem) { return up(rows * up(cols, vec_of(elem)) * elem_bytes(elem), 16) / 4; }
 
-// The tile and the number of splits of the contraction, by the time a model gives them (cycles):
-//   rounds of tiles on a compute unit x (steps x the slower of products and loads + a fixed part)
-//   + writing and reading the splits' sums.
-// Rates are of the tile kernel on its own (bf16 8192^3: 256 x 256 1310 TFLOP/s, 128 x 128 900), a load
-// costs a compute unit a cycle per 24 bytes.
-struct Tile { int bm, bn; float rate16, rate32; };  // share of the peak rate
-constexpr Tile TILES[] = {{256, 256, 0.72f, 0.0f}, {128, 128, 0.60f, 0.80f}, {128, 64, 0.50f, 0.86f},
-                          {64, 64, 0.40f, 0.90f},  {128, 32, 0.35f, 0.88f},  {32, 128, 0.35f, 0.86f}};
+// The tile and the number of splits of the contraction, by the time (cycles) that a model of a compute
+// unit's share gives them: `at_once` workgroups of a tile fit its LDS and take turns at the matrix
+// units, a step of theirs takes the slowest of the products, the loads and the loads' latency; splits
+// add the writing and joining of their sums.  The numbers are fitted to 3273 measured times of 26
+// shapes' three products, 6 tiles and 1 to 256 splits: the model's choice is 2.3% (16-bit) and 1.5%
+// (f32) slower than the fastest measured on average, 14% and 22% at worst.  A product at the wrong end
+// of the list loses much more: dw of 158976 x 224 x 32 in f32 takes 3100 us unsplit and 63 us in 256.
+struct Tile { int bm, bn, at_once; double rate16, rate32; };  // rates: shares of 4096, 256 operations a cycle
+constexpr Tile TILES[] = {{256, 256, 1, 0.66, 0.0}, {128, 128, 2, 0.62, 0.86}, {128, 64, 3, 0.30, 0.88},
+                          {64, 64, 5, 0.33, 0.88},  {128, 32, 4, 0.17, 0.82},  {32, 128, 4, 0.24, 0.85}};
+struct Cost { double load, latency, fixed, epilogue, more, join, join_byte; };
+constexpr Cost COST16 = {1.0 / 26, 2300, 200, 0.16, 1.6, 16000, 1.0 / 710};
+constexpr Cost COST32 = {0, 1400, 0, 0, 1, 3200, 1.0 / 1800};
 struct Shape { int tile, tiles_m, tiles_n, splits, kchunk; };
 
 Shape shape_of(int M, int N, int K, int elem) {
   const bool wide = elem == GWN_ELEM_F32;
+  const Cost& co = wide ? COST32 : COST16;
   const int bk = wide ? 32 : 64;
   const long cus = gwn_device_cus(), steps = (K + bk - 1) / bk;
   Shape best{};
   double least = 1e300;
   for (int t = 0; t < 6; ++t) {
     const Tile& c = TILES[t];
-    const double rate = wide ? c.rate32 * 256.0 : c.rate16 * 4096.0;
-    if (rate == 0.0) continue;
+    const double rate = wide ? c.rate32 * 256 : c.rate16 * 4096;
+    if (rate == 0) continue;
     const long tm = (M + c.bm - 1) / c.bm, tn = (N + c.bn - 1) / c.bn, tiles = tm * tn;
-    const double product = 2.0 * c.bm * c.bn * bk / rate, loads = (c.bm + c.bn) * 128.0 / 24.0;
-    const double step = product > loads ? product : loads;
+    const double product = 2.0 * c.bm * c.bn * bk / rate, loads = (c.bm + c.bn) * 128 * co.load;
+    const double step = product > loads ? product : loads, fixed = co.fixed + c.bm * c.bn * co.epilogue;
     long last = 0;
     for (long want = 1; want <= 512; want += (want + 3) / 4) {
       const long chunk = (steps + want - 1) / want, splits = chunk ? (steps + chunk - 1) / chunk : 1;
       if (splits == last) continue;
       last = splits;
-      const long rounds = (tiles * splits + cus - 1) / cus;
-      const double join = splits > 1 ? 8000.0 + 8.0 * M * N * splits / 2000.0 : 0.0;
-      const double time = rounds * (chunk * step + 2000.0 + c.bm * c.bn / 6.0) + join;
+      const long share = (tiles * splits + cus - 1) / cus, full = share / c.at_once, rest = share % c.at_once;
+      const double all = c.at_once * step, some = rest * step;
+      double time = full * ((all > co.latency ? all : co.latency) * chunk + fixed * co.more);
+      if (rest) time += (some > co.latency ? some : co.latency) * chunk + fixed;
+      if (splits > 1) time += co.join + 8.0 * M * N * splits * co.join_byte;
       if (time < least) {
         least = time;
         best = {t, (int)tm, (int)tn, (int)splits, (int)(chunk * bk)};
@@ -673,7 +761,10 @@ int copy_rows(const void* x, long ld, long rows, int cols, float*& at, int elem,
   return GWN_OK;
 }
 
+bool few_rows(const gwn_linear_args* a) { return a->M <= 32; }
+
 long fwd_floats(const gwn_linear_args* a) {
+  if (few_rows(a)) return 0;
   long f = part_floats(a->M, a->N, a->K, a->elem);
   if (!stageable(a->x, a->ldx, a->K, a->elem)) f += copy_floats(a->M, a->K, a->elem);
   if (!stageable(a->w, a->ldw, a->K, a->elem)) f += copy_floats(a->N, a->K, a->elem);
@@ -682,6 +773,19 @@ long fwd_floats(const gwn_linear_args* a) {
 
 template <typename T>
 int fwd(const gwn_linear_args* a, hipStream_t s) {
+  const Epi e{a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->y, a->ldy, a->N, a->act,
+              drop_of(a->seed_ptr, a->salt, a->drop_p)};
+  if (few_rows(a)) {
+    const Few p{a->x, a->ldx, a->w, a->ldw, a->M, a->N, a->K, e};
+    const int turn = 16 * vec_of(a->elem), turns = (a->K + turn - 1) / turn;  // contraction values a wave takes at once
+    const int threads = 64 * (turns < 16 ? turns : 16), grid = (a->N + 15) / 16;
+    if (a->M <= 16)
+      few_kernel<T, 1><<<grid, threads, 0, s>>>(p);
+    else
+      few_kernel<T, 2><<<grid, threads, 0, s>>>(p);
+    GWN_CHECK_LAUNCH();
+    return GWN_OK;
+  }
   Operand x{a->x, a->ldx}, w{a->w, a->ldw};
   float* at = a->workspace;
   if (!stageable(a->x, a->ldx, a->K, a->elem)) {
@@ -692,8 +796,6 @@ int fwd(const gwn_linear_args* a, hipStream_t s) {
     const int rc = copy_rows<T>(a->w, a->ldw, a->N, a->K, at, a->elem, w, s);
     if (rc) return rc;
   }
-  const Epi e{a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->y, a->ldy, a->N, a->act,
-              drop_of(a->seed_ptr, a->salt, a->drop_p)};
   const int kp = (int)up(a->K, vec_of(a->elem));  // a copy's zeros included
   return gemm<T>(K_ROWS, K_ROWS, x, w, a->M, a->N, kp, kp, a->elem, e, at, s);
 }
