@@ -58,85 +58,163 @@ __device__ __forceinline__ void store_f(T* p, const float (&v)[V], int rem) {
   }
 }
 
-// sum over the G lanes of a group, the same value in all of them
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* lds) {
-#pragma unroll
-  for (int o = 1; o < (G < 64 ? G : 64); o <<= 1) v += __shfl_xor(v, o, 64);
-  if (G > 64) {
-    __syncthreads();  // the last sum's reads are done
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) v += lds[w];
-  }
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over G lanes of a wave, the same value in all of them: neighbours, pairs, the halves of 8 and of
+// 16 by mirrored lane operands, 16s and 32s by shuffles
+template <int G> __device__ __forceinline__ float lanes_sum(float v) {
+  if (G >= 2) v += dpp<0xB1>(v);
+  if (G >= 4) v += dpp<0x4E>(v);
+  if (G >= 8) v += dpp<0x141>(v);
+  if (G >= 16) v += dpp<0x140>(v);
+  if (G >= 32) v += __shfl_xor(v, 16, 64);
+  if (G >= 64) v += __shfl_xor(v, 32, 64);
   return v;
+}
+// sums over the G lanes of a group, the same values in all of them.  A workgroup's go through `lds`, one
+// barrier: the caller alternates between two areas, so that an area is written again only behind the
+// other's barrier, which all its readers have reached.
+template <int G, int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float (*lds)[4]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = lanes_sum<(G < 64 ? G : 64)>(v[k]);
+  if (G > 64) {
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) lds[k][threadIdx.x >> 6] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = lds[k][0] + lds[k][1] + lds[k][2] + lds[k][3];
+  }
+}
+
+// A lane's vectors of a row.  Vector i starts at column at(i); where it would reach over the row's end it
+// starts V columns before the end, and its first cut(i) values, another lane's too, are left out of the
+// sums: no load is predicated by element.  (Rows shorter than a vector are.)
+template <int V, int G>
+struct Span {
+  int c, lane;
+  __device__ __forceinline__ int whole(int i) const { return (lane + G * i) * V; }
+  __device__ __forceinline__ int at(int i) const {
+    const int w = whole(i);
+    return c < V ? 0 : w + V <= c ? w : c - V;
+  }
+  __device__ __forceinline__ int cut(int i) const { return c < V ? 0 : whole(i) - at(i); }
+  __device__ __forceinline__ bool in(int i) const { return whole(i) < c; }
+  // whether value j of vector i counts: always, but in the row's last round of vectors
+  __device__ __forceinline__ bool counts(int i, int j) const {
+    if (G * (i + 1) * V <= c) return true;
+    return c < V ? lane + G * i == 0 && j < c : j >= cut(i);
+  }
+  template <typename T> __device__ __forceinline__ Pack<T, V> get(const T* row, int i) const {
+    if (c >= V) return load<T, V>(row + at(i));
+    Pack<T, V> a;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.v[j] = j < c ? row[j] : (T)0.0f;
+    return a;
+  }
+  template <typename T> __device__ __forceinline__ void put(T* row, int i, const float (&v)[V]) const {
+    if (!in(i)) return;
+    if (c >= V) {
+      Pack<T, V> a;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a.v[j] = (T)v[j];
+      store<T, V>(row + at(i), a);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < c) row[j] = (T)v[j];
+    }
+  }
+};
+
+// the parameters' vectors as floats (`none` where there are no parameters)
+template <typename W, int V, int G>
+__device__ __forceinline__ void params_of(float (&o)[V], const Span<V, G>& sp, const void* p, int i, float none) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = none;
+    return;
+  }
+  const Pack<W, V> a = sp.template get<W>((const W*)p, i);
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = (float)a.v[j];
 }
 
 template <typename T, typename W, int G, int I>
 __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const LnFwd p) {
-  constexpr int V = Vec<T>::N;
-  __shared__ float red[THREADS / 64];
-  const int lane = threadIdx.x % G;
+  constexpr int V = Vec<T>::N, PER = THREADS / G;
+  constexpr bool HOLD = I * V <= 16;  // the parameters stay in registers over the rows
+  __shared__ float red[2][2][4];
+  const Span<V, G> sp{p.c, (int)threadIdx.x % G};
   const float c = (float)p.c;
-  constexpr int PER = THREADS / G;
   const long step = (long)gridDim.x * PER;
-  // whole groups leave together; a whole workgroup where the group is one
-  for (long row = (long)blockIdx.x * PER + threadIdx.x / G; row < p.rows; row += step) {
-    const T* x = (const T*)p.x + row * p.ldx;
-    float v[I][V], sum = 0.0f;
+  float g[I][V], b[I][V];
+  if (HOLD) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int at = (lane + G * i) * V;
-      load_f<T, V>(v[i], x + at, p.c - at, 0.0f);
+      params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
+      params_of<W, V, G>(b[i], sp, p.beta, i, 0.0f);
     }
+  }
+  long row = (long)blockIdx.x * PER + threadIdx.x / G;
+  Pack<T, V> next[I];
+  if (row < p.rows)
+#pragma unroll
+    for (int i = 0; i < I; ++i) next[i] = sp.template get<T>((const T*)p.x + row * p.ldx, i);
+  // whole groups leave together; a whole workgroup where the group is one
+  for (; row < p.rows; row += step) {
+    float v[I][V], s[1] = {0.0f}, d[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += v[i][j];
-    float mean = group_sum<G>(sum, red) / c, sq = 0.0f, sd = 0.0f;
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = (float)next[i].v[j];
+        s[0] += sp.counts(i, j) ? v[i][j] : 0.0f;
+      }
+    if (row + step < p.rows)  // the next row's loads are in flight during this row's sums
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const int rem = p.c - (lane + G * i) * V;
+      for (int i = 0; i < I; ++i) next[i] = sp.template get<T>((const T*)p.x + (row + step) * p.ldx, i);
+    group_sums<G, 1>(s, red[0]);
+    const float mean = s[0] / c;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] = j < rem ? v[i][j] - mean : 0.0f;
-        sq += v[i][j] * v[i][j];
-        sd += v[i][j];
+        v[i][j] -= mean;
+        const float w = sp.counts(i, j) ? v[i][j] : 0.0f;
+        d[0] += w;
+        d[1] += w * w;
       }
-    }
-    const float left = group_sum<G>(sd, red) / c;
-    const float rstd = 1.0f / sqrtf(fmaxf(group_sum<G>(sq, red) / c - left * left, 0.0f) + p.eps);
-    mean += left;
-    if (p.mean && lane == 0) {
-      p.mean[row] = mean;
+    group_sums<G, 2>(d, red[1]);
+    const float left = d[0] / c;
+    const float rstd = 1.0f / sqrtf(fmaxf(d[1] / c - left * left, 0.0f) + p.eps);
+    if (p.mean && sp.lane == 0) {
+      p.mean[row] = mean + left;
       p.rstd[row] = rstd;
     }
-    T* y = (T*)p.y + row * p.ldy;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int at = (lane + G * i) * V, rem = p.c - at;
-      if (rem > 0) {
-        float o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = (v[i][j] - left) * rstd;
-        if (p.gamma) {
-          float g[V];
-          load_f<W, V>(g, (const W*)p.gamma + at, rem, 0.0f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) o[j] *= g[j];
-        }
-        if (p.beta) {
-          float b[V];
-          load_f<W, V>(b, (const W*)p.beta + at, rem, 0.0f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) o[j] += b[j];
-        }
-        store_f<T, V>(y + at, o, rem);
+      if (!HOLD) {
+        params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
+        params_of<W, V, G>(b[i], sp, p.beta, i, 0.0f);
       }
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = (v[i][j] - left) * rstd * g[i][j] + b[i][j];
+      sp.template put<T>((T*)p.y + row * p.ldy, i, o);
     }
   }
+}
+
+// one sum over a workgroup
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+  v = lanes_sum<64>(v);
+  __syncthreads();  // the last sum's reads are done
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
 // rows of any length, a workgroup each: three passes over a row
@@ -155,7 +233,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_long_kernel(const LnFwd p) {
 #pragma unroll
       for (int j = 0; j < V; ++j) sum += v[j];
     }
-    const float first = group_sum<THREADS>(sum, red) / c;
+    const float first = block_sum(sum, red) / c;
     for (long at = (long)threadIdx.x * V; at < p.c; at += THREADS * V) {
       float v[V];
       load_f<T, V>(v, x + at, (int)(p.c - at), first);
@@ -166,8 +244,8 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_long_kernel(const LnFwd p) {
         sd += d;
       }
     }
-    const float left = group_sum<THREADS>(sd, red) / c, mean = first + left;
-    const float rstd = 1.0f / sqrtf(fmaxf(group_sum<THREADS>(sq, red) / c - left * left, 0.0f) + p.eps);
+    const float left = block_sum(sd, red) / c, mean = first + left;
+    const float rstd = 1.0f / sqrtf(fmaxf(block_sum(sq, red) / c - left * left, 0.0f) + p.eps);
     if (p.mean && threadIdx.x == 0) {
       p.mean[row] = mean;
       p.rstd[row] = rstd;
@@ -192,71 +270,81 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_long_kernel(const LnFwd p) {
 template <typename T, typename W, int G, int I>
 __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const LnBwd p) {
   constexpr int V = Vec<T>::N, PER = THREADS / G;
-  __shared__ float red[THREADS / 64];
+  constexpr bool HOLD = I * V <= 16;
+  __shared__ float red[2][2][4];
   __shared__ float cols[PER > 1 ? 2 * G * I * V : 1];
-  const int lane = threadIdx.x % G;
+  const Span<V, G> sp{p.c, (int)threadIdx.x % G};
   const float inv = 1.0f / (float)p.c;
-  float dg[I][V] = {}, db[I][V] = {};
+  float dg[I][V] = {}, db[I][V] = {}, g[I][V];
+  if (HOLD)
+#pragma unroll
+    for (int i = 0; i < I; ++i) params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
   const long step = (long)gridDim.x * PER;
-  for (long row = (long)blockIdx.x * PER + threadIdx.x / G; row < p.rows; row += step) {
-    const T* x = (const T*)p.x + row * p.ldx;
-    const T* dy = (const T*)p.dy + row * p.ld_dy;
-    const float mean = p.mean[row], rstd = p.rstd[row];
-    float v[I][V], h[I][V], s1 = 0.0f, s2 = 0.0f;
+  long row = (long)blockIdx.x * PER + threadIdx.x / G;
+  Pack<T, V> nx[I], ny[I];
+  float nmean = 0.0f, nrstd = 0.0f;
+  auto fetch = [&](long r) {
+    nmean = p.mean[r], nrstd = p.rstd[r];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int at = (lane + G * i) * V, rem = p.c - at;
-      load_f<T, V>(v[i], x + at, rem, mean);
-      load_f<T, V>(h[i], dy + at, rem, 0.0f);
+      nx[i] = sp.template get<T>((const T*)p.x + r * p.ldx, i);
+      ny[i] = sp.template get<T>((const T*)p.dy + r * p.ld_dy, i);
     }
+  };
+  if (row < p.rows) fetch(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    const float mean = nmean, rstd = nrstd;
+    float v[I][V], h[I][V], s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const int at = (lane + G * i) * V, rem = p.c - at;
-      float g[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) g[j] = 1.0f;
-      if (p.gamma && rem > 0) load_f<W, V>(g, (const W*)p.gamma + at, rem, 0.0f);
+    for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] = (v[i][j] - mean) * rstd;
-        dg[i][j] += h[i][j] * v[i][j];
+        v[i][j] = ((float)nx[i].v[j] - mean) * rstd;
+        h[i][j] = (float)ny[i].v[j];
+      }
+    if (row + step < p.rows) fetch(row + step);
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      if (!HOLD) params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        dg[i][j] += h[i][j] * v[i][j];  // of a cut vector's first values another lane has the sums
         db[i][j] += h[i][j];
-        h[i][j] *= g[j];
-        s1 += h[i][j];
-        s2 += h[i][j] * v[i][j];
+        h[i][j] *= g[i][j];
+        const float w = sp.counts(i, j) ? h[i][j] : 0.0f;
+        s[0] += w;
+        s[1] += sp.counts(i, j) ? w * v[i][j] : 0.0f;
       }
     }
     if (!p.dx) continue;
-    s1 = group_sum<G>(s1, red) * inv;
-    s2 = group_sum<G>(s2, red) * inv;
-    T* dx = (T*)p.dx + row * p.ld_dx;
+    group_sums<G, 2>(s, red[turn]);
+    const float s1 = s[0] * inv, s2 = s[1] * inv;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int at = (lane + G * i) * V, rem = p.c - at;
       float o[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = rstd * (h[i][j] - s1 - v[i][j] * s2);
-      if (rem > 0) store_f<T, V>(dx + at, o, rem);
+      sp.template put<T>((T*)p.dx + row * p.ld_dx, i, o);
     }
   }
   if (!p.part) return;
   float* part = p.part + (long)blockIdx.x * 2 * p.c;
   if constexpr (PER == 1) {
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const int at = (lane + G * i) * V, rem = p.c - at;
-      if (rem > 0) {
-        store_f<float, V>(part + at, dg[i], rem);
-        store_f<float, V>(part + p.c + at, db[i], rem);
-      }
-    }
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (sp.in(i) && sp.counts(i, j)) {
+          part[sp.at(i) + j] = dg[i][j];
+          part[p.c + sp.at(i) + j] = db[i][j];
+        }
   } else {
     // a wave's groups by shuffles, then the waves one after the other
-  #pragma unroll
+#pragma unroll
     for (int i = 0; i < I; ++i)
-  #pragma unroll
+#pragma unroll
       for (int j = 0; j < V; ++j)
-  #pragma unroll
+#pragma unroll
         for (int o = G; o < 64; o <<= 1) {
           dg[i][j] += __shfl_xor(dg[i][j], o, 64);
           db[i][j] += __shfl_xor(db[i][j], o, 64);
@@ -265,14 +353,15 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const LnBwd p) {
     for (int w = 0; w < THREADS / 64; ++w) {
       __syncthreads();
       if (wave == w && (threadIdx.x & 63) < G) {
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < I; ++i)
-  #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int at = (lane + G * i) * V + j;
-            cols[at] = w ? cols[at] + dg[i][j] : dg[i][j];
-            cols[G * I * V + at] = w ? cols[G * I * V + at] + db[i][j] : db[i][j];
-          }
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (sp.in(i) && sp.counts(i, j)) {
+              const int at = sp.at(i) + j;
+              cols[at] = w ? cols[at] + dg[i][j] : dg[i][j];
+              cols[G * I * V + at] = w ? cols[G * I * V + at] + db[i][j] : db[i][j];
+            }
       }
     }
     __syncthreads();
@@ -320,8 +409,8 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_long_kernel(const LnBwd p) {
         }
       }
       if (pass == 0) {
-        s1 = group_sum<THREADS>(s1, red) * inv;
-        s2 = group_sum<THREADS>(s2, red) * inv;
+        s1 = block_sum(s1, red) * inv;
+        s2 = block_sum(s2, red) * inv;
       }
     }
   }
@@ -411,7 +500,7 @@ int vectors(int c, int elem) { return (int)(((long)c * elem_bytes(elem) + 15) / 
 // workgroups of the backward, each with one partial row
 int bwd_grid(long rows, int c, int elem) {
   const Group g = group_of(vectors(c, elem));
-  const long most = (long)gwn_device_cus() * 2;
+  const long most = (long)gwn_device_cus() * (c >= 2048 ? 2 : 4);
   if (!g.G) {
     const long by = (rows + 15) / 16;
     return (int)(by < 1 ? 1 : by < 64 ? by : 64);
@@ -423,7 +512,7 @@ int bwd_grid(long rows, int c, int elem) {
 template <typename T, typename W>
 int fwd(const LnFwd& p, int elem, hipStream_t s) {
   const Group g = group_of(vectors(p.c, elem));
-  const long per = g.G ? THREADS / g.G : 1, want = (p.rows + per - 1) / per, most = (long)gwn_device_cus() * 16;
+  const long per = g.G ? THREADS / g.G : 1, want = (p.rows + per - 1) / per, most = (long)gwn_device_cus() * 8;
   const int grid = (int)(want < most ? want : most);
 #define X(GG, II)                                            \
   if (g.G == GG && g.I == II) {                              \
