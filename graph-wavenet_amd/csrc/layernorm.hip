@@ -5,8 +5,8 @@
 //   dg = sum_rows dy xh,  db = sum_rows dy
 //
 // Bound by memory: x read and y written once forward; x and dy read, dx written once backward.  A
-// row lives in the registers of a group of G lanes (G = 4 .. 64 lanes of a wave, or a whole
-// workgroup), I 16-byte vectors a lane, so that the variance is the centred sum of squares and
+// row lives in the registers of a group of G lanes (G = 4 .. 64 lanes of a wave, or a workgroup of as
+// many waves as its 16-byte vectors need), one vector a lane, so that the variance is the centred sum of squares and
 // nothing is read twice.  The centred values' own mean is taken off again (the corrected two-pass
 // form): the first mean's rounding, which 1 / sqrt(eps) would magnify in a row that hardly varies,
 // drops out, and a constant row gives exactly b.  Groups walk the rows; each lane keeps its columns' sums of dg and db in
@@ -19,7 +19,7 @@ using namespace elem;
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, MOST = 1024;  // a workgroup's, of small groups and at most
 
 struct LnFwd {
   const void* x; long ldx; long rows; int c;
@@ -72,66 +72,77 @@ template <int G> __device__ __forceinline__ float lanes_sum(float v) {
   if (G >= 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
-// sums over the G lanes of a group, the same values in all of them.  A workgroup's go through `lds`, one
-// barrier: the caller alternates between two areas, so that an area is written again only behind the
-// other's barrier, which all its readers have reached.
+// Sums over the lanes of a group (G = 0: a workgroup), the same values in all of them.  A workgroup's go
+// through `lds`, one barrier: the caller alternates between two areas, so that an area is written again
+// only behind the other's barrier, which all its readers have reached.
 template <int G, int N>
-__device__ __forceinline__ void group_sums(float (&v)[N], float (*lds)[4]) {
+__device__ __forceinline__ void group_sums(float (&v)[N], float (*lds)[MOST / 64]) {
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = lanes_sum<(G < 64 ? G : 64)>(v[k]);
-  if (G > 64) {
+  for (int k = 0; k < N; ++k) v[k] = lanes_sum<(G ? G : 64)>(v[k]);
+  if (G == 0) {
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int k = 0; k < N; ++k) lds[k][threadIdx.x >> 6] = v[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = lds[k][0] + lds[k][1] + lds[k][2] + lds[k][3];
+    for (int k = 0; k < N; ++k) {
+      v[k] = 0.0f;
+      for (int w = 0; w < (int)blockDim.x >> 6; ++w) v[k] += lds[k][w];
+    }
   }
 }
 
-// A lane's vectors of a row.  Vector i starts at column at(i); where it would reach over the row's end it
-// starts V columns before the end, and its first cut(i) values, another lane's too, are left out of the
-// sums: no load is predicated by element.  (Rows shorter than a vector are.)
-template <int V, int G>
+// A lane's vectors of a row, I of them.  EVEN: the row is whole vectors, lanes past its end have none.
+// Otherwise the vector that would reach over the row's end starts V columns before the end, and its
+// first cut(i) values, another lane's too, are left out of the sums: no load is predicated by element
+// (but in rows shorter than a vector).
+template <int V, int G, bool EVEN>
 struct Span {
   int c, lane;
-  __device__ __forceinline__ int whole(int i) const { return (lane + G * i) * V; }
+  static constexpr bool TINY = !EVEN && G == 4;  // rows shorter than a vector are among these
+  __device__ __forceinline__ int whole(int i) const { return (lane + (int)blockDim.x * i) * V; }
+  __device__ __forceinline__ bool in(int i) const { return whole(i) < c; }
   __device__ __forceinline__ int at(int i) const {
     const int w = whole(i);
-    return c < V ? 0 : w + V <= c ? w : c - V;
+    if (EVEN) return w;
+    return TINY && c < V ? 0 : w + V <= c ? w : c - V;
   }
-  __device__ __forceinline__ int cut(int i) const { return c < V ? 0 : whole(i) - at(i); }
-  __device__ __forceinline__ bool in(int i) const { return whole(i) < c; }
-  // whether value j of vector i counts: always, but in the row's last round of vectors
-  __device__ __forceinline__ bool counts(int i, int j) const {
-    if (G * (i + 1) * V <= c) return true;
-    return c < V ? lane + G * i == 0 && j < c : j >= cut(i);
+  // whether value j of vector i, which is in the row, is this lane's
+  __device__ __forceinline__ bool own(int i, int j) const {
+    if (EVEN) return true;
+    return TINY && c < V ? j < c : j >= whole(i) - at(i);
   }
+  __device__ __forceinline__ bool counts(int i, int j) const { return in(i) && own(i, j); }
+  // zeros where there is no vector
   template <typename T> __device__ __forceinline__ Pack<T, V> get(const T* row, int i) const {
-    if (c >= V) return load<T, V>(row + at(i));
-    Pack<T, V> a;
+    Pack<T, V> a{};
+    if (TINY && c < V) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = j < c ? row[j] : (T)0.0f;
+      for (int j = 0; j < V; ++j)
+        if (in(i) && j < c) a.v[j] = row[j];
+    } else if (in(i)) {
+      a = load<T, V>(row + at(i));
+    }
     return a;
   }
   template <typename T> __device__ __forceinline__ void put(T* row, int i, const float (&v)[V]) const {
     if (!in(i)) return;
-    if (c >= V) {
+    if (TINY && c < V) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < c) row[j] = (T)v[j];
+    } else {
       Pack<T, V> a;
 #pragma unroll
       for (int j = 0; j < V; ++j) a.v[j] = (T)v[j];
       store<T, V>(row + at(i), a);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < c) row[j] = (T)v[j];
     }
   }
 };
 
 // the parameters' vectors as floats (`none` where there are no parameters)
-template <typename W, int V, int G>
-__device__ __forceinline__ void params_of(float (&o)[V], const Span<V, G>& sp, const void* p, int i, float none) {
+template <typename W, int V, typename S>
+__device__ __forceinline__ void params_of(float (&o)[V], const S& sp, const void* p, int i, float none) {
   if (!p) {
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = none;
@@ -142,23 +153,24 @@ __device__ __forceinline__ void params_of(float (&o)[V], const Span<V, G>& sp, c
   for (int j = 0; j < V; ++j) o[j] = (float)a.v[j];
 }
 
-template <typename T, typename W, int G, int I>
-__global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const LnFwd p) {
-  constexpr int V = Vec<T>::N, PER = THREADS / G;
-  constexpr bool HOLD = I * V <= 16;  // the parameters stay in registers over the rows
-  __shared__ float red[2][2][4];
-  const Span<V, G> sp{p.c, (int)threadIdx.x % G};
+template <typename T, typename W, int G, int I, bool EVEN>
+__global__ __launch_bounds__(G ? THREADS : I == 1 ? MOST : MOST / 2) void ln_fwd_kernel(const LnFwd p) {
+  constexpr int V = Vec<T>::N, PER = G ? THREADS / (G ? G : 1) : 1;
+  static_assert(G == 0 || I == 1, "one vector a lane");
+  constexpr bool HOLD = I == 1;  // the parameters stay in registers over the rows
+  __shared__ float red[2][2][MOST / 64];
+  const Span<V, G, EVEN> sp{p.c, G ? (int)threadIdx.x % (G ? G : 1) : (int)threadIdx.x};
   const float c = (float)p.c;
   const long step = (long)gridDim.x * PER;
   float g[I][V], b[I][V];
   if (HOLD) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
-      params_of<W, V, G>(b[i], sp, p.beta, i, 0.0f);
+      params_of<W, V>(g[i], sp, p.gamma, i, 1.0f);
+      params_of<W, V>(b[i], sp, p.beta, i, 0.0f);
     }
   }
-  long row = (long)blockIdx.x * PER + threadIdx.x / G;
+  long row = (long)blockIdx.x * PER + (G ? threadIdx.x / (G ? G : 1) : 0);
   Pack<T, V> next[I];
   if (row < p.rows)
 #pragma unroll
@@ -171,7 +183,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const LnFwd p) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         v[i][j] = (float)next[i].v[j];
-        s[0] += sp.counts(i, j) ? v[i][j] : 0.0f;
+        s[0] += sp.own(i, j) ? v[i][j] : 0.0f;  // zeros where there is no vector
       }
     if (row + step < p.rows)  // the next row's loads are in flight during this row's sums
 #pragma unroll
@@ -197,8 +209,8 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const LnFwd p) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       if (!HOLD) {
-        params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
-        params_of<W, V, G>(b[i], sp, p.beta, i, 0.0f);
+        params_of<W, V>(g[i], sp, p.gamma, i, 1.0f);
+        params_of<W, V>(b[i], sp, p.beta, i, 0.0f);
       }
       float o[V];
 #pragma unroll
@@ -267,20 +279,21 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_long_kernel(const LnFwd p) {
   }
 }
 
-template <typename T, typename W, int G, int I>
-__global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const LnBwd p) {
-  constexpr int V = Vec<T>::N, PER = THREADS / G;
-  constexpr bool HOLD = I * V <= 16;
-  __shared__ float red[2][2][4];
-  __shared__ float cols[PER > 1 ? 2 * G * I * V : 1];
-  const Span<V, G> sp{p.c, (int)threadIdx.x % G};
+template <typename T, typename W, int G, int I, bool EVEN>
+__global__ __launch_bounds__(G ? THREADS : I == 1 ? MOST : MOST / 2) void ln_bwd_kernel(const LnBwd p) {
+  constexpr int V = Vec<T>::N, PER = G ? THREADS / (G ? G : 1) : 1;
+  static_assert(G == 0 || I == 1, "one vector a lane");
+  constexpr bool HOLD = I == 1;
+  __shared__ float red[2][2][MOST / 64];
+  __shared__ float cols[PER > 1 ? 2 * G * V : 1];
+  const Span<V, G, EVEN> sp{p.c, G ? (int)threadIdx.x % (G ? G : 1) : (int)threadIdx.x};
   const float inv = 1.0f / (float)p.c;
   float dg[I][V] = {}, db[I][V] = {}, g[I][V];
   if (HOLD)
 #pragma unroll
-    for (int i = 0; i < I; ++i) params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
+    for (int i = 0; i < I; ++i) params_of<W, V>(g[i], sp, p.gamma, i, 1.0f);
   const long step = (long)gridDim.x * PER;
-  long row = (long)blockIdx.x * PER + threadIdx.x / G;
+  long row = (long)blockIdx.x * PER + (G ? threadIdx.x / (G ? G : 1) : 0);
   Pack<T, V> nx[I], ny[I];
   float nmean = 0.0f, nrstd = 0.0f;
   auto fetch = [&](long r) {
@@ -305,15 +318,15 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const LnBwd p) {
     if (row + step < p.rows) fetch(row + step);
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      if (!HOLD) params_of<W, V, G>(g[i], sp, p.gamma, i, 1.0f);
+      if (!HOLD) params_of<W, V>(g[i], sp, p.gamma, i, 1.0f);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         dg[i][j] += h[i][j] * v[i][j];  // of a cut vector's first values another lane has the sums
         db[i][j] += h[i][j];
         h[i][j] *= g[i][j];
-        const float w = sp.counts(i, j) ? h[i][j] : 0.0f;
+        const float w = sp.own(i, j) ? h[i][j] : 0.0f;  // zeros where there is no vector
         s[0] += w;
-        s[1] += sp.counts(i, j) ? w * v[i][j] : 0.0f;
+        s[1] += w * v[i][j];
       }
     }
     if (!p.dx) continue;
@@ -331,13 +344,19 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const LnBwd p) {
   float* part = p.part + (long)blockIdx.x * 2 * p.c;
   if constexpr (PER == 1) {
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+    for (int i = 0; i < I; ++i) {
+      if (EVEN) {
+        sp.template put<float>(part, i, dg[i]);
+        sp.template put<float>(part + p.c, i, db[i]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (sp.in(i) && sp.counts(i, j)) {
-          part[sp.at(i) + j] = dg[i][j];
-          part[p.c + sp.at(i) + j] = db[i][j];
-        }
+        for (int j = 0; j < V; ++j)
+          if (sp.counts(i, j)) {
+            part[sp.at(i) + j] = dg[i][j];
+            part[p.c + sp.at(i) + j] = db[i][j];
+          }
+      }
+    }
   } else {
     // a wave's groups by shuffles, then the waves one after the other
 #pragma unroll
@@ -357,17 +376,17 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const LnBwd p) {
         for (int i = 0; i < I; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if (sp.in(i) && sp.counts(i, j)) {
+            if (sp.counts(i, j)) {
               const int at = sp.at(i) + j;
               cols[at] = w ? cols[at] + dg[i][j] : dg[i][j];
-              cols[G * I * V + at] = w ? cols[G * I * V + at] + db[i][j] : db[i][j];
+              cols[G * V + at] = w ? cols[G * V + at] + db[i][j] : db[i][j];
             }
       }
     }
     __syncthreads();
     for (int k = threadIdx.x; k < p.c; k += THREADS) {
       part[k] = cols[k];
-      part[p.c + k] = cols[G * I * V + k];
+      part[p.c + k] = cols[G * V + k];
     }
   }
 }
@@ -478,45 +497,45 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* part, int 
   }
 }
 
-// the group that holds a row of n vectors: lanes G and vectors a lane I; G = 0: too long
-struct Group { int G, I; };
-Group group_of(int n) {
-  if (n <= 4) return {4, 1};
-  if (n <= 8) return {8, 1};
-  if (n <= 16) return {16, 1};
-  if (n <= 32) return {32, 1};
-  if (n <= 256) return {64, (n + 63) / 64};
-  const int i = (n + 255) / 256;
-  if (i <= 4) return {256, i};
-  if (i <= 6) return {256, 6};
-  if (i <= 8) return {256, 8};
-  return {0, 0};
+// How rows of n vectors are held: by groups of G lanes, or (G = 0) a workgroup of `threads`, I vectors a
+// lane; I = 0: too long.  The backward's grid, each workgroup of which writes a partial row, is what a
+// compute unit's registers hold at once (16-bit elements 20 waves, f32 32; 4 workgroups of small groups).
+struct Group { int G, I, threads, at_once; };
+Group group_of(int n, int elem) {
+  const int waves = elem == GWN_ELEM_F32 ? 32 : 20;
+  for (int g = 4; g <= 64; g *= 2)
+    if (n <= g) return {g, 1, THREADS, 4};
+  const int w = (n + 63) / 64;
+  if (w <= MOST / 64) return {0, 1, w * 64, waves / w > 0 ? waves / w : 1};
+  if (w <= MOST / 64 * 2) return {0, 4, MOST / 2, 1};
+  return {0, 0, THREADS, 0};
 }
 int vectors(int c, int elem) { return (int)(((long)c * elem_bytes(elem) + 15) / 16); }
 
-#define LN_GROUPS(X) \
-  X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 3) X(64, 4) X(256, 2) X(256, 3) X(256, 4) X(256, 6) X(256, 8)
+#define LN_GROUPS(X) X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(0, 1) X(0, 4)
 
 // workgroups of the backward, each with one partial row
 int bwd_grid(long rows, int c, int elem) {
-  const Group g = group_of(vectors(c, elem));
-  const long most = (long)gwn_device_cus() * (c >= 2048 ? 2 : 4);
-  if (!g.G) {
+  const Group g = group_of(vectors(c, elem), elem);
+  if (!g.I) {
     const long by = (rows + 15) / 16;
     return (int)(by < 1 ? 1 : by < 64 ? by : 64);
   }
-  const long per = THREADS / g.G, want = (rows + per - 1) / per;
+  const long most = (long)gwn_device_cus() * g.at_once;
+  const long per = g.G ? THREADS / g.G : 1, want = (rows + per - 1) / per;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 template <typename T, typename W>
 int fwd(const LnFwd& p, int elem, hipStream_t s) {
-  const Group g = group_of(vectors(p.c, elem));
-  const long per = g.G ? THREADS / g.G : 1, want = (p.rows + per - 1) / per, most = (long)gwn_device_cus() * 8;
+  const Group g = group_of(vectors(p.c, elem), elem);
+  const long per = g.G ? THREADS / g.G : 1, want = (p.rows + per - 1) / per;
+  const long most = (long)gwn_device_cus() * (2048 / g.threads);
   const int grid = (int)(want < most ? want : most);
+  const bool even = p.c % Vec<T>::N == 0;
 #define X(GG, II)                                            \
   if (g.G == GG && g.I == II) {                              \
-    ln_fwd_kernel<T, W, GG, II><<<grid, THREADS, 0, s>>>(p); \
+    (even ? ln_fwd_kernel<T, W, GG, II, true> : ln_fwd_kernel<T, W, GG, II, false>)<<<grid, g.threads, 0, s>>>(p); \
     GWN_CHECK_LAUNCH();                                      \
     return GWN_OK;                                           \
   }
@@ -529,12 +548,13 @@ int fwd(const LnFwd& p, int elem, hipStream_t s) {
 
 template <typename T, typename W>
 int bwd(const LnBwd& p, int elem, void* dgamma, void* dbeta, hipStream_t s) {
-  const Group g = group_of(vectors(p.c, elem));
+  const Group g = group_of(vectors(p.c, elem), elem);
   const int grid = bwd_grid(p.rows, p.c, elem);
   bool done = p.rows == 0;
+  const bool even = p.c % Vec<T>::N == 0;
 #define X(GG, II)                                            \
   if (!done && g.G == GG && g.I == II) {                     \
-    ln_bwd_kernel<T, W, GG, II><<<grid, THREADS, 0, s>>>(p); \
+    (even ? ln_bwd_kernel<T, W, GG, II, true> : ln_bwd_kernel<T, W, GG, II, false>)<<<grid, g.threads, 0, s>>>(p); \
     GWN_CHECK_LAUNCH();                                      \
     done = true;                                             \
   }

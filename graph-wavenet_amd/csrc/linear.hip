@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
 // v_mfma_f32_16x16x32 (16-bit) or 16x16x4 fragments.  A workgroup has 16 columns (w rows), its waves
 // split the contraction: 4 loads of 16 bytes a lane, 256 bytes of each w row, are in flight a wave and
 // turn, x's pieces come from the caches.  The waves' sums meet in LDS, then the epilogue.  Rows may
-// start anywhere; a piece over the contraction's end is loaded by element.
+// start anywhere and have any length.
 struct Few {
   const void* x; long ldx;
   const void* w; long ldw;
@@ -487,12 +487,20 @@ __device__ __forceinline__ f32x4 mma16(Pack<float, 4> a, Pack<float, 4> b, f32x4
   for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
   return c;
 }
+// a row's values k .. k + V - 1.  Where they would reach over the row's end K, the V values before the
+// end, those before k as zeros: the contraction's order does not matter as long as x and w share it
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_part(const T* p, int rem) {
-  if (rem >= V) return load<T, V>(p);
+__device__ __forceinline__ Pack<T, V> load_end(const T* row, int k, int K) {
   Pack<T, V> a;
+  if (K >= V) {
+    const int at = k + V <= K ? k : K - V;
+    a = load<T, V>(row + at);
 #pragma unroll
-  for (int j = 0; j < V; ++j) a.v[j] = j < rem ? p[j] : (T)0.0f;
+    for (int j = 0; j < V; ++j) a.v[j] = at + j >= k ? a.v[j] : (T)0.0f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.v[j] = k + j < K ? row[k + j] : (T)0.0f;
+  }
   return a;
 }
 
@@ -511,12 +519,20 @@ __global__ __launch_bounds__(1024) void few_kernel(const Few p) {
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int k0 = wave * KS * U; k0 < p.K; k0 += waves * KS * U) {
     Pack<T, V> a[U], b[MT][U];
+    if (k0 + KS * U <= p.K) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * KS + kl;
-      a[u] = load_part<T, V>(w + k, p.K - k);
+      for (int u = 0; u < U; ++u) {
+        a[u] = load<T, V>(w + k0 + u * KS + kl);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) b[i][u] = load_part<T, V>(x[i] + k, p.K - k);
+        for (int i = 0; i < MT; ++i) b[i][u] = load<T, V>(x[i] + k0 + u * KS + kl);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        a[u] = load_end<T, V>(w, k0 + u * KS + kl, p.K);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) b[i][u] = load_end<T, V>(x[i], k0 + u * KS + kl, p.K);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
