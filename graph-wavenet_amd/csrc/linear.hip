@@ -777,7 +777,13 @@ int copy_rows(const void* x, long ld, long rows, int cols, float*& at, int elem,
   return GWN_OK;
 }
 
-bool few_rows(const gwn_linear_args* a) { return a->M <= 32; }
+// Where the few-rows kernel is the faster one.  Its workgroups take 2048 (16-bit) or 1024 (f32) values of
+// the contraction a turn and read x again each: 1 x 1024 x 4096 in bf16 4.1 us against the tiles' 7.5, 32 x
+// 1024 x 4096 5.8 against 9.1, 16 x 4096 x 4096 11.2 against 13.7; but 16 x 8192 x 512 16.5 against 8.6, 24 x
+// 4096 x 2048 13.8 against 11.7, 16 x 4096 x 16384 40 against 31.
+bool few_rows(const gwn_linear_args* a) {
+  return a->M <= 32 && (long)a->M * a->N <= 131072 && a->K <= (a->M <= 16 ? 4096 : 1024);
+}
 
 long fwd_floats(const gwn_linear_args* a) {
   if (few_rows(a)) return 0;
