@@ -16,6 +16,7 @@ The tensors of one call share a device and a type (layer norm's parameters may s
 is queued on that device's current stream.  Inputs may be strided over their leading axes; where
 the last axis is not contiguous or the leading axes do not fold into rows, a copy is made.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -73,19 +74,12 @@ def _stream(t):
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-class _on:
-    """t's device as the current one during a call (nothing to do where it is already)."""
+_NO_GUARD = contextlib.nullcontext()
 
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on(t):
+    """t's device as the current one during a call (autograd's threads have it set already)."""
+    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _backward(impl):
@@ -139,10 +133,9 @@ def _linear_bwd(ctx, dy):
     a = _lib.LinearBwdArgs(dy.data_ptr(), ldy, ptr(x), ldx, ptr(weight), ldw, ptr(z), n, ptr(dx), k, ptr(dw), k, ptr(db), m,
                            n, k, _ELEM[dy.dtype], ctx.act, ptr(seed), ctx.salt, ctx.p, None)
     at = ctypes.byref(a)
-    with _on(dy):
-        ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(at), dy)
-        a.workspace = ptr(ws)
-        _lib.call("gwn_linear_bwd", at, _stream(dy))
+    ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(at), dy)
+    a.workspace = ptr(ws)
+    _lib.call("gwn_linear_bwd", at, _stream(dy))
     return dx, dw, db, dres, None, None, None, None
 
 
@@ -168,7 +161,8 @@ def linear_act(x, weight, bias=None, act="none", residual=None, p=0.0, seed=None
     _check("linear_act", x, weight, bias, residual)
     if act not in ACTS:
         raise ValueError("linear_act: act must be one of %s, got %r" % (", ".join(ACTS), act))
-    _check_seed("linear_act", x, p, seed, salt)
+    if p != 0.0:
+        _check_seed("linear_act", x, p, seed, salt)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise RuntimeError("linear_act: x [..., K] and weight [N, K] do not fit: %s, %s"
                            % (tuple(x.shape), tuple(weight.shape)))
@@ -207,26 +201,20 @@ def _norm_fwd(x, weight, bias, eps, keep):
 
 
 def _norm_bwd(ctx, dy):
+    # the thread that runs this starts cold: what the forward can prepare is in ctx.plan
     x, weight, stats = ctx.saved_tensors
-    c = x.shape[-1]
-    m = x.numel() // c
+    m, c, elem, params, floats = ctx.plan
     needs = ctx.needs_input_grad
-    pt = ctx.params_dtype
     dx = x.new_empty(x.shape) if needs[0] else None
-    dw = x.new_empty(c, dtype=pt) if needs[1] else None
-    db = x.new_empty(c, dtype=pt) if needs[2] else None
+    dw = x.new_empty(c, dtype=params) if needs[1] else None
+    db = x.new_empty(c, dtype=params) if needs[2] else None
+    ws = x.new_empty(floats, dtype=F32) if needs[1] or needs[2] else None
     x, ldx = _rows(x, c)
     dy, ldy = _rows(dy, c)
     weight = weight.contiguous() if weight is not None else None
-    elem = _ELEM[x.dtype]
-    mean = stats.data_ptr()
-    with _on(x):
-        ws = None
-        if dw is not None or db is not None:
-            ws = _ws(_lib.load().gwn_layernorm_bwd_workspace_floats(m, c, elem), x)
-        _lib.call("gwn_layernorm_bwd", dy.data_ptr(), ldy, x.data_ptr(), ldx, m, c, elem, _lib.ptr(weight),
-                  int(pt == F32), mean, mean + 4 * m, _lib.ptr(dx), c, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws),
-                  _stream(x))
+    mean, ptr = stats.data_ptr(), _lib.ptr
+    _lib.call("gwn_layernorm_bwd", dy.data_ptr(), ldy, x.data_ptr(), ldx, m, c, elem, ptr(weight), int(params == F32), mean,
+              mean + 4 * m, ptr(dx), c, ptr(dw), ptr(db), ptr(ws), _stream(x))
     return dx, dw, db, None
 
 
@@ -236,7 +224,12 @@ class _LayerNormFn(torch.autograd.Function):
         y, stats = _norm_fwd(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
         params = weight if weight is not None else bias
-        ctx.params_dtype = None if params is None else params.dtype
+        c, elem = x.shape[-1], _ELEM[x.dtype]
+        m = x.numel() // c
+        floats = 0
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            floats = _lib.load().gwn_layernorm_bwd_workspace_floats(m, c, elem)
+        ctx.plan = m, c, elem, None if params is None else params.dtype, floats
         return y
 
     backward = _backward(_norm_bwd)
@@ -270,10 +263,14 @@ def _drop(x, residual, p, seed, salt):
     y = x.new_empty(x.shape)
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None
-    with _on(x):
-        _lib.call("gwn_dropout", x.data_ptr(), _lib.ptr(residual), y.data_ptr(), y.numel(), _ELEM[x.dtype],
-                  seed.data_ptr(), salt, p, _stream(x))
+    _lib.call("gwn_dropout", x.data_ptr(), _lib.ptr(residual), y.data_ptr(), y.numel(), _ELEM[x.dtype], seed.data_ptr(),
+              salt, p, _stream(x))
     return y
+
+
+def _drop_fwd(x, residual, p, seed, salt):
+    with _on(x):
+        return _drop(x, residual, p, seed, salt)
 
 
 def _drop_bwd(ctx, dy):
@@ -287,7 +284,7 @@ class _DropoutFn(torch.autograd.Function):
     def forward(ctx, x, residual, p, seed, salt):
         ctx.save_for_backward(seed)
         ctx.p, ctx.salt = p, salt
-        return _drop(x, residual, p, seed, salt)
+        return _drop_fwd(x, residual, p, seed, salt)
 
     backward = _backward(_drop_bwd)
 
@@ -308,7 +305,7 @@ def dropout(x, p, seed, salt=0, residual=None):
         return x.clone() if residual is None else x + residual
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _DropoutFn.apply(x, residual, float(p), seed, salt)
-    return _drop(x, residual, float(p), seed, salt)
+    return _drop_fwd(x, residual, float(p), seed, salt)
 
 
 # ---- modules --------------------------------------------------------------------------------
