@@ -16,7 +16,6 @@ The tensors of one call share a device and a type (layer norm's parameters may s
 is queued on that device's current stream.  Inputs may be strided over their leading axes; where
 the last axis is not contiguous or the leading axes do not fold into rows, a copy is made.
 """
-import contextlib
 import ctypes
 
 import torch
@@ -68,18 +67,25 @@ def _ws(floats, like):
     return like.new_empty(floats, dtype=F32) if floats > 0 else None
 
 
-def _stream(t):
-    """The raw handle of the current stream of t's device (a tenth of a microsecond; a Stream object
-    built for its handle costs up to 15, as much as a small kernel's whole launch)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+# The raw stream handle and the current device without the Python objects around them: building a
+# Stream for its handle costs up to 15 us in a step, as much as a small kernel's whole launch.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
 
 
-_NO_GUARD = contextlib.nullcontext()
+def _here(t):
+    """Whether t's device is the current one (in autograd's threads it always is)."""
+    return t.device.index == _device()
 
 
-def _on(t):
-    """t's device as the current one during a call (autograd's threads have it set already)."""
-    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _elsewhere(fn):
+    """``fn`` (its first argument a tensor) on that tensor's device."""
+    def run(t, *args):
+        if _here(t):
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+    return run
 
 
 def _backward(impl):
@@ -91,6 +97,7 @@ def _backward(impl):
 
 # ---- the product with its epilogue ----------------------------------------------------------
 
+@_elsewhere
 def _linear_fwd(x, weight, bias, act, residual, p, seed, salt, keep_z):
     n, k = weight.shape
     y = x.new_empty(x.shape[:-1] + (n,))
@@ -108,10 +115,10 @@ def _linear_fwd(x, weight, bias, act, residual, p, seed, salt, keep_z):
     a = _lib.LinearArgs(x.data_ptr(), ldx, weight.data_ptr(), ldw, ptr(bias), ptr(residual), ldr, y.data_ptr(), n, ptr(z), n,
                         m, n, k, _ELEM[x.dtype], act, seed.data_ptr() if p > 0.0 else None, salt, p, None)
     at = ctypes.byref(a)
-    with _on(x):
-        ws = _ws(_lib.load().gwn_linear_fwd_workspace_floats(at), x)
-        a.workspace = ptr(ws)
-        _lib.call("gwn_linear_fwd", at, _stream(x))
+    ws = _ws(_lib.load().gwn_linear_fwd_workspace_floats(at), x)
+    if ws is not None:
+        a.workspace = ws.data_ptr()
+    _lib.call("gwn_linear_fwd", at, _raw_stream(x.device.index))
     return y, z
 
 
@@ -121,7 +128,7 @@ def _linear_bwd(ctx, dy):
     needs = ctx.needs_input_grad
     dres = dy if needs[3] else None
     if not (needs[0] or needs[1] or needs[2]):
-        return None, None, None, dres, None, None, None, None
+        return None, None, None, dres, None
     dx = dy.new_empty(ctx.shape) if needs[0] else None
     dw = dy.new_empty((n, k)) if needs[1] else None
     db = dy.new_empty(n) if needs[2] else None
@@ -135,13 +142,14 @@ def _linear_bwd(ctx, dy):
     at = ctypes.byref(a)
     ws = _ws(_lib.load().gwn_linear_bwd_workspace_floats(at), dy)
     a.workspace = ptr(ws)
-    _lib.call("gwn_linear_bwd", at, _stream(dy))
-    return dx, dw, db, dres, None, None, None, None
+    _lib.call("gwn_linear_bwd", at, _raw_stream(dy.device.index))
+    return dx, dw, db, dres, None
 
 
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, p, seed, salt):
+    def forward(ctx, x, weight, bias, residual, how):
+        act, p, seed, salt = how
         needs = ctx.needs_input_grad
         y, z = _linear_fwd(x, weight, bias, act, residual, p, seed, salt, needs[0] or needs[1] or needs[2])
         ctx.save_for_backward(x if needs[1] else None, weight if needs[0] else None, z, seed if p > 0.0 else None)
@@ -166,7 +174,10 @@ def linear_act(x, weight, bias=None, act="none", residual=None, p=0.0, seed=None
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise RuntimeError("linear_act: x [..., K] and weight [N, K] do not fit: %s, %s"
                            % (tuple(x.shape), tuple(weight.shape)))
-    n = weight.shape[0]
+    n, k = weight.shape
+    if max(n, k) > 2 ** 20 or x.numel() > k * 2 ** 30:
+        raise RuntimeError("linear_act: at most 2^30 rows and 2^20 channels, got %s, %s"
+                           % (tuple(x.shape), tuple(weight.shape)))
     if bias is not None and bias.shape != (n,):
         raise RuntimeError("linear_act: bias must be [%d], got %s" % (n, tuple(bias.shape)))
     if residual is not None and residual.shape != x.shape[:-1] + (n,):
@@ -175,29 +186,30 @@ def linear_act(x, weight, bias=None, act="none", residual=None, p=0.0, seed=None
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
-        return _LinearActFn.apply(x, weight, bias, residual, ACTS[act], float(p), seed, salt)
+        return _LinearActFn.apply(x, weight, bias, residual, (ACTS[act], float(p), seed, salt))
     return _linear_fwd(x, weight, bias, ACTS[act], residual, float(p), seed, salt, False)[0]
 
 
 # ---- layer norm -----------------------------------------------------------------------------
 
+@_elsewhere
 def _norm_fwd(x, weight, bias, eps, keep):
-    c = x.shape[-1]
+    """y, the rows' statistics if they are to be kept, and the backward's workspace floats."""
+    c, elem = x.shape[-1], _ELEM[x.dtype]
     y = x.new_empty(x.shape)
     m = x.numel() // c
     stats = x.new_empty((2, m), dtype=F32) if keep else None
-    if m == 0:
-        return y, stats
     x, ldx = _rows(x, c)
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
     params = weight if weight is not None else bias
     wide = int(params is not None and params.dtype == F32)
     mean = stats.data_ptr() if keep else None
-    with _on(x):
-        _lib.call("gwn_layernorm_fwd", x.data_ptr(), ldx, m, c, _ELEM[x.dtype], _lib.ptr(weight), _lib.ptr(bias),
-                  wide, eps, y.data_ptr(), c, mean, mean + 4 * m if keep else None, _stream(x))
-    return y, stats
+    if m:
+        _lib.call("gwn_layernorm_fwd", x.data_ptr(), ldx, m, c, elem, _lib.ptr(weight), _lib.ptr(bias), wide, eps,
+                  y.data_ptr(), c, mean, mean + 4 * m if keep else None, _raw_stream(x.device.index))
+    floats = _lib.load().gwn_layernorm_bwd_workspace_floats(m, c, elem) if keep else 0
+    return y, stats, floats
 
 
 def _norm_bwd(ctx, dy):
@@ -214,22 +226,17 @@ def _norm_bwd(ctx, dy):
     weight = weight.contiguous() if weight is not None else None
     mean, ptr = stats.data_ptr(), _lib.ptr
     _lib.call("gwn_layernorm_bwd", dy.data_ptr(), ldy, x.data_ptr(), ldx, m, c, elem, ptr(weight), int(params == F32), mean,
-              mean + 4 * m, ptr(dx), c, ptr(dw), ptr(db), ptr(ws), _stream(x))
+              mean + 4 * m, ptr(dx), c, ptr(dw), ptr(db), ptr(ws), _raw_stream(x.device.index))
     return dx, dw, db, None
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = _norm_fwd(x, weight, bias, eps, True)
+        y, stats, floats = _norm_fwd(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
         params = weight if weight is not None else bias
-        c, elem = x.shape[-1], _ELEM[x.dtype]
-        m = x.numel() // c
-        floats = 0
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            floats = _lib.load().gwn_layernorm_bwd_workspace_floats(m, c, elem)
-        ctx.plan = m, c, elem, None if params is None else params.dtype, floats
+        ctx.plan = stats.shape[1], x.shape[-1], _ELEM[x.dtype], None if params is None else params.dtype, floats
         return y
 
     backward = _backward(_norm_bwd)
@@ -241,8 +248,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     weight and bias ``[C]`` (either may be None) have x's type, or are both float32.  Differentiable in
     x, weight and bias."""
     _check("layer_norm", x)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise RuntimeError("layer_norm: x must be [..., C] with C > 0, got %s" % (tuple(x.shape),))
+    if x.dim() < 1 or not 0 < x.shape[-1] <= 2 ** 30:
+        raise RuntimeError("layer_norm: x must be [..., C] with 0 < C <= 2^30, got %s" % (tuple(x.shape),))
     if not eps >= 0.0:
         raise ValueError("layer_norm: eps must not be negative, got %s" % eps)
     params = [t for t in (weight, bias) if t is not None]
@@ -264,24 +271,23 @@ def _drop(x, residual, p, seed, salt):
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None
     _lib.call("gwn_dropout", x.data_ptr(), _lib.ptr(residual), y.data_ptr(), y.numel(), _ELEM[x.dtype], seed.data_ptr(),
-              salt, p, _stream(x))
+              salt, p, _raw_stream(x.device.index))
     return y
 
 
-def _drop_fwd(x, residual, p, seed, salt):
-    with _on(x):
-        return _drop(x, residual, p, seed, salt)
+_drop_fwd = _elsewhere(_drop)
 
 
 def _drop_bwd(ctx, dy):
     needs = ctx.needs_input_grad
     dx = _drop(dy, None, ctx.p, ctx.saved_tensors[0], ctx.salt) if needs[0] else None
-    return dx, (dy if needs[1] else None), None, None, None
+    return dx, (dy if needs[1] else None), None
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, salt):
+    def forward(ctx, x, residual, how):
+        p, seed, salt = how
         ctx.save_for_backward(seed)
         ctx.p, ctx.salt = p, salt
         return _drop_fwd(x, residual, p, seed, salt)
@@ -304,7 +310,7 @@ def dropout(x, p, seed, salt=0, residual=None):
     if p == 0.0:
         return x.clone() if residual is None else x + residual
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _DropoutFn.apply(x, residual, float(p), seed, salt)
+        return _DropoutFn.apply(x, residual, (float(p), seed, salt))
     return _drop_fwd(x, residual, float(p), seed, salt)
 
 

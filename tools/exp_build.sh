@@ -19,8 +19,8 @@ HIPCC=/opt/rocm/bin/hipcc
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-result -I$ROOT/include"
 pids=()
 for f in $(cd "$D/g/csrc" && ls *.hip | sed 's/\.hip$//'); do
-  fl="$FLAGS"  # as build.sh: no packed fp32 ops in the GCN tile kernels
-  case " gcn_fused gcn_slice " in *" $f "*) fl="$FLAGS -Xclang -target-feature -Xclang -packed-fp32-ops" ;; esac
+  fl="$FLAGS"  # as build.sh: no packed fp32 ops in the GCN tile kernels and the position-wise layers
+  case " gcn_fused gcn_slice linear layernorm dropout " in *" $f "*) fl="$FLAGS -Xclang -target-feature -Xclang -packed-fp32-ops" ;; esac
   $HIPCC $fl -c -o "$D/$f.o" "$D/g/csrc/$f.hip" 2>/dev/null & pids+=($!)
 done
 for p in "${pids[@]}"; do wait "$p"; done
