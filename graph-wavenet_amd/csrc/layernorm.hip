@@ -561,13 +561,13 @@ int bwd(const LnBwd& p, int elem, void* dgamma, void* dbeta, hipStream_t s) {
   LN_GROUPS(X)
 #undef X
   if (!done) {
+    if (p.part) {  // first: dx may overwrite dy
+      ln_cols_long_kernel<T><<<dim3((vectors(p.c, elem) + 63) / 64, grid), THREADS, 0, s>>>(p);
+      GWN_CHECK_LAUNCH();
+    }
     if (p.dx) {
       const long most = (long)gwn_device_cus() * 8;
       ln_bwd_long_kernel<T, W><<<(int)(p.rows < most ? p.rows : most), THREADS, 0, s>>>(p);
-      GWN_CHECK_LAUNCH();
-    }
-    if (p.part) {
-      ln_cols_long_kernel<T><<<dim3((vectors(p.c, elem) + 63) / 64, grid), THREADS, 0, s>>>(p);
       GWN_CHECK_LAUNCH();
     }
   }
