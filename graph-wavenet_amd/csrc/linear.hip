@@ -618,10 +618,14 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
       for (int u = 0; u < 2; ++u) {
         const long r = m + u * TY;
         if (r >= last) break;
+        if (ACT != GWN_ACT_NONE) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[u][j] *= act_slope<is16<T>, ACT>(z[u][j]);
+        }
+        // last, so that a dropped element's dz is 0 whatever dy and z hold there
         if (p.drop.thr) drop_vec<V>(v[u], key, p.drop, (unsigned long long)r * p.N + n);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (ACT != GWN_ACT_NONE) v[u][j] *= act_slope<is16<T>, ACT>(z[u][j]);
           if (j >= rem) v[u][j] = 0.0f;
           sum[j] += v[u][j];
         }

@@ -817,7 +817,8 @@ int gwn_linear_fwd(const gwn_linear_args* a, hipStream_t stream);
 long gwn_linear_fwd_workspace_floats(const gwn_linear_args* a);
 
 /* Gradients of gwn_linear_fwd, each NULL = not wanted (dresidual is dy itself):
- *   dz = D'(dy) act'(z) (rounded to the element type where act or dropout make it differ from dy),
+ *   dz = D'(dy act'(z)) (rounded to the element type where act or dropout make it differ from dy; 0
+ *   where dropout dropped, whatever dy and z hold there),
  *   dx = dz w, dw = dz^T x, dbias = sum_m dz (of the unrounded dz).
  * act, seed, salt and drop_p as the forward had them. */
 typedef struct gwn_linear_bwd_args {

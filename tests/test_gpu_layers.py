@@ -561,7 +561,202 @@ def test_rows_past_32_bits(gpu):
         assert torch.equal(a, b)
 
 
+def test_outputs_past_32_bits(gpu):
+    """More than 2^32 outputs: the last rows' values, mask and gradients are those of a small call (whose
+    mask the oracle moves to the same elements)."""
+    from gwn_amd.layers import linear_act
+    m, k, n = 4200000, 32, 1032
+    c = LinearCase(40, k, n, "bf16", "relu", True, False, 0.5)
+    x = torch.zeros(m, k, device=gpu, dtype=torch.bfloat16)
+    x[-40:] = c.x.to(gpu)
+    x.requires_grad_()
+    w, b = c.w.to(gpu), c.b.to(gpu)
+    seed = torch.tensor([c.seed], device=gpu)
+    y = linear_act(x, w, b, act="relu", p=0.5, seed=seed, salt=c.salt)
+    assert y.numel() > 2 ** 32
+    keep = mask(c.seed, c.salt, (40, n), 0.5, (m - 40) * n)
+    z = c.x.double() @ c.w.double().T + c.b.double()  # exact: on grids
+    want = torch.where(keep, z.clamp(min=0) * 2, torch.zeros((), dtype=F64))
+    assert torch.equal(y[-40:].cpu(), want.to(torch.bfloat16))
+    dy = torch.zeros_like(y)
+    dy[-40:] = c.dy.to(gpu)
+    dx, = torch.autograd.grad(y, x, dy)
+    dz = torch.where(keep & (z > 0), c.dy.double() * 2, torch.zeros((), dtype=F64))
+    want = dz @ c.w.double()
+    within("dx", dx[-40:], want, (n + 2) * E32 * (dz.abs() @ c.w.double().abs())
+           + half_step("bf16") * want.abs() * (1 + 2.0 ** -8) + TINY["bf16"])
+    assert not dx[:-40].any()
+
+
+def test_norm_past_32_bits(gpu):
+    from gwn_amd.layers import layer_norm
+    m, c = 1050000, 4096
+    x, w, b, dy = norm_inputs(8, c, "bf16", True)
+    big = torch.empty(m, c, device=gpu, dtype=torch.bfloat16)
+    big[:] = x[0].to(gpu)
+    big[-8:] = x.to(gpu)
+    big.requires_grad_()
+    y = layer_norm(big, w.to(gpu), b.to(gpu))
+    g = torch.zeros_like(y)
+    g[-8:] = dy.to(gpu)
+    dx, = torch.autograd.grad(y, big, g)
+    norm_check("bf16", x, w, b, dy, 1e-5, y[-8:], dx[-8:])
+    assert not dx[:-8].any() and torch.equal(y[0], y[m // 2])
+
+
+# ---- the C entries ----------------------------------------------------------------------------
+
+def fenced(rows, cols, ld, t, dev, fill):
+    """A [rows][ld] buffer of ``fill`` whose first cols columns are a matrix."""
+    return torch.full((rows, ld), fill, device=dev, dtype=t)
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("m,k,n", [(5, 40, 36), (70, 41, 67), (300, 128, 200)])
+def test_linear_entries_leave_the_rest(gpu, t, m, k, n):
+    """Every leading dimension longer than its row: what lies behind the rows stays as it was, also
+    with the debugging checks of ranges on."""
+    import ctypes
+    from gwn_amd import _lib
+    lib, dt, elem = _lib.load(), TYPES[t], {"f32": 0, "f16": 1, "bf16": 2}[t]
+    zt = torch.float32 if t == "f32" else torch.float16
+    c = LinearCase(m, k, n, t, "silu", True, True, 0.3)
+    x, w, r = (fenced(a, b_, b_ + 5, dt, gpu, math.nan) for a, b_ in ((m, k), (n, k), (m, n)))
+    x[:, :k], w[:, :k], r[:, :n] = c.x.to(gpu), c.w.to(gpu), c.r.to(gpu)
+    dyb = fenced(m, n, n + 3, dt, gpu, math.nan)
+    dyb[:, :n] = c.dy.to(gpu)
+    b, seed = c.b.to(gpu), torch.tensor([c.seed], device=gpu)
+    y, z = fenced(m, n, n + 7, dt, gpu, 7.0), fenced(m, n, n + 1, zt, gpu, 7.0)
+    dx, dw, db = fenced(m, k, k + 2, dt, gpu, 7.0), fenced(n, k, k + 9, dt, gpu, 7.0), torch.empty(n, device=gpu, dtype=dt)
+    st = torch.cuda.current_stream().cuda_stream
+    f = _lib.LinearArgs(x.data_ptr(), k + 5, w.data_ptr(), k + 5, b.data_ptr(), r.data_ptr(), n + 5, y.data_ptr(), n + 7,
+                        z.data_ptr(), n + 1, m, n, k, elem, 4, seed.data_ptr(), c.salt, 0.3, None)
+    g = _lib.LinearBwdArgs(dyb.data_ptr(), n + 3, x.data_ptr(), k + 5, w.data_ptr(), k + 5, z.data_ptr(), n + 1,
+                           dx.data_ptr(), k + 2, dw.data_ptr(), k + 9, db.data_ptr(), m, n, k, elem, 4, seed.data_ptr(),
+                           c.salt, 0.3, None)
+    ws = [torch.full((max(1, v),), math.nan, device=gpu) for v in
+          (lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f)), lib.gwn_linear_bwd_workspace_floats(ctypes.byref(g)))]
+    f.workspace, g.workspace = ws[0].data_ptr(), ws[1].data_ptr()
+    lib.gwn_set_sync_check(1)
+    try:
+        _lib.check(lib.gwn_linear_fwd(ctypes.byref(f), st))
+        _lib.check(lib.gwn_linear_bwd(ctypes.byref(g), st))
+    finally:
+        lib.gwn_set_sync_check(0)
+    c.check(y=y[:, :n], dx=dx[:, :k], dw=dw[:, :k], db=db)
+    for v, cols in ((y, n), (z, n), (dx, k), (dw, k)):
+        assert (v[:, cols:] == 7.0).all()
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("c", [6, 33, 600, 9000, 40000])
+def test_norm_entries_in_place(gpu, t, c):
+    """y over x and dx over dy, rows apart, what lies between them as it was."""
+    from gwn_amd import _lib
+    lib, elem, m = _lib.load(), {"f32": 0, "f16": 1, "bf16": 2}[t], 11
+    x, w, b, dy = norm_inputs(m, c, t, False)
+    xd, yd, gd = (fenced(m, c, c + 3, TYPES[t], gpu, 7.0) for _ in range(3))
+    xd[:, :c], yd[:, :c], gd[:, :c] = x.to(gpu), x.to(gpu), dy.to(gpu)
+    wd, bd, stats = w.to(gpu), b.to(gpu), torch.empty(2, m, device=gpu)
+    dw, db = torch.empty_like(wd), torch.empty_like(bd)
+    ws = torch.full((lib.gwn_layernorm_bwd_workspace_floats(m, c, elem),), math.nan, device=gpu)
+    st, mean = torch.cuda.current_stream().cuda_stream, stats.data_ptr()
+    lib.gwn_set_sync_check(1)
+    try:
+        _lib.check(lib.gwn_layernorm_fwd(yd.data_ptr(), c + 3, m, c, elem, wd.data_ptr(), bd.data_ptr(), int(t == "f32"), 1e-5,
+                                         yd.data_ptr(), c + 3, mean, mean + 4 * m, st))
+        _lib.check(lib.gwn_layernorm_bwd(gd.data_ptr(), c + 3, xd.data_ptr(), c + 3, m, c, elem, wd.data_ptr(),
+                                         int(t == "f32"), mean, mean + 4 * m, gd.data_ptr(), c + 3, dw.data_ptr(),
+                                         db.data_ptr(), ws.data_ptr(), st))
+    finally:
+        lib.gwn_set_sync_check(0)
+    norm_check(t, x, w, b, dy, 1e-5, yd[:, :c], gd[:, :c], dw, db)
+    assert (yd[:, c:] == 7.0).all() and (gd[:, c:] == 7.0).all()
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+def test_dropout_entry_in_place(gpu, t):
+    from gwn_amd import _lib
+    from gwn_amd.layers import dropout
+    elem = {"f32": 0, "f16": 1, "bf16": 2}[t]
+    x, r = torch.randn(5003, device=gpu).to(TYPES[t]), torch.randn(5003, device=gpu).to(TYPES[t])
+    seed = torch.tensor([8], device=gpu)
+    want = dropout(x, 0.3, seed, salt=2, residual=r)
+    st = torch.cuda.current_stream().cuda_stream
+    for into in (0, 1):
+        a, b = torch.cat([x, x[:9]]), torch.cat([r, r[:9]])
+        y = (a, b)[into]
+        _lib.call("gwn_dropout", a.data_ptr(), b.data_ptr(), y.data_ptr(), 5003, elem, seed.data_ptr(), 2, 0.3, st)
+        assert torch.equal(y[:5003], want) and torch.equal(y[5003:], (x, r)[into][:9])
+
+
 # ---- together ---------------------------------------------------------------------------------
+
+def test_one_tensor_twice(gpu):
+    """The input as its own residual and weight: the gradients add up."""
+    from gwn_amd.layers import linear_act
+    x = torch.randn(48, 48, device=gpu, requires_grad=True)
+    dy = torch.randn(48, 48, device=gpu)
+    gx, = torch.autograd.grad(linear_act(x, x, act="gelu", residual=x), x, dy)
+    parts = [x.detach().clone().requires_grad_() for _ in range(3)]
+    apart = torch.autograd.grad(linear_act(parts[0], parts[1], act="gelu", residual=parts[2]), parts, dy)
+    want = sum(v.double() for v in apart)
+    assert float((gx.double() - want).abs().max()) <= 4 * E32 * float(sum(v.abs() for v in apart).max())
+
+
+def test_dropped_places_hide_nan_backward(gpu):
+    """Where dropout dropped, neither a NaN pre-activation nor a NaN gradient gets through."""
+    from gwn_amd.layers import dropout, linear_act
+    seed = torch.tensor([13], device=gpu)
+    x = torch.randn(64, 32, device=gpu)
+    w = torch.randn(80, 32, device=gpu)
+    b = torch.zeros(80, device=gpu)
+    keep = mask(13, 0, (64, 80), 0.5).to(gpu)
+    clean = []
+    for bad in (False, True):
+        xs = x.clone().requires_grad_()
+        res = torch.zeros(64, 80, device=gpu)
+        y = linear_act(xs, w, b, act="gelu", p=0.5, seed=seed, residual=res)
+        dy = torch.ones(64, 80, device=gpu)
+        if bad:
+            dy[~keep] = math.nan
+        clean.append(torch.autograd.grad(y, xs, dy)[0])
+    assert torch.isfinite(clean[1]).all() and torch.equal(clean[0], clean[1])
+    # a bias of NaN in one column: only rows that keep it see it
+    b[3] = math.nan
+    xs = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(linear_act(xs, w, b, act="gelu", p=0.5, seed=seed), xs, torch.ones(64, 80, device=gpu))
+    assert torch.equal(torch.isfinite(dx).all(1), ~keep[:, 3])
+    xs = x.clone().requires_grad_()
+    y = dropout(xs, 0.5, seed)
+    dy = torch.ones_like(y)
+    dy[y == 0] = math.inf
+    assert torch.isfinite(torch.autograd.grad(y, xs, dy)[0]).all()
+
+
+def test_two_streams_at_once(gpu):
+    from gwn_amd.layers import layer_norm
+    c = LinearCase(3000, 256, 512, "bf16", "gelu", True, False, 0.2)
+    (x, w, b, _), dy, seed = c.on(gpu)
+    from gwn_amd.layers import linear_act
+    g = torch.ones(512, device=gpu, dtype=torch.bfloat16, requires_grad=True)
+
+    def work():
+        y = layer_norm(linear_act(x, w, b, act="gelu", p=0.2, seed=seed, salt=c.salt), g)
+        return [y] + list(torch.autograd.grad(y, (x, w, b, g), dy))
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for r in got:
+        for p, q in zip(want, r):
+            assert torch.equal(p, q)
 
 @pytest.mark.parametrize("t", sorted(TYPES))
 def test_epilogue_mask_is_dropouts(gpu, t):
