@@ -584,7 +584,8 @@ struct Dz {
   const void* dy; long ld_dy;
   const void* z; long ldz;
   void* dz; int ld;  // [M][ld], columns past N zero; NULL = not written
-  float* part;       // [gridDim.y][N] column sums, NULL = not wanted
+  float* part;       // [gridDim.y][N] column sums (one stripe: none), and
+  void* db;          // where one stripe's go; both NULL = not wanted
   int M, N, tx, stripe;  // TX = 1 << tx; rows a workgroup
   Drop drop;
 };
@@ -632,7 +633,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
         if (p.dz) store_f<T, V>((T*)p.dz + r * p.ld + n, v[u], V);
       }
     }
-  if (!p.part) return;
+  if (!p.db) return;
 #pragma unroll
   for (int j = 0; j < V; ++j) cols[threadIdx.x * V + j] = sum[j];
   __syncthreads();
@@ -641,7 +642,10 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
     if (at < p.N) {
       float v = 0.0f;
       for (int q = 0; q < TY; ++q) v += cols[q * TX * V + k];
-      p.part[(long)blockIdx.y * p.N + at] = v;
+      if (gridDim.y == 1)
+        ((T*)p.db)[at] = (T)v;
+      else
+        p.part[(long)blockIdx.y * p.N + at] = v;
     }
   }
 }
@@ -845,10 +849,10 @@ BwdPlan bwd_plan(const gwn_linear_bwd_args* a) {
   long parts = (8L * gwn_device_cus() + bx - 1) / bx, most = (a->M + 4 * ty - 1) / (4 * ty);
   if (parts > most) parts = most;
   if (parts > 1024) parts = 1024;
-  if (parts < 1) parts = 1;
+  if (parts < 1 || a->M <= 16 * ty) parts = 1;  // few rows: a launch less
   q.stripe = (int)up((a->M + parts - 1) / parts, 2 * ty);
   q.parts = a->M ? (a->M + q.stripe - 1) / q.stripe : 1;
-  q.floats = a->dbias ? up((long)q.parts * a->N, 4) : 0;
+  q.floats = a->dbias && q.parts > 1 ? up((long)q.parts * a->N, 4) : 0;
   if (q.write_dz) q.floats += copy_floats(a->M, a->N, a->elem);
   if (q.copy_x) q.floats += copy_floats(a->M, a->K, a->elem);
   if (q.copy_w) q.floats += copy_floats(a->N, a->K, a->elem);
@@ -868,14 +872,14 @@ int bwd(const gwn_linear_bwd_args* a, hipStream_t s) {
   const Drop drop = drop_of(a->seed_ptr, a->salt, a->drop_p);
   float* at = a->workspace;
   float* sums = at;
-  if (a->dbias) at += up((long)q.parts * a->N, 4);
+  if (a->dbias && q.parts > 1) at += up((long)q.parts * a->N, 4);
   Operand dz{a->dy, a->ld_dy}, x{a->x, a->ldx}, w{a->w, a->ldw};
   if (q.write_dz) {
     dz = {at, q.ld_dz};
     at += copy_floats(a->M, a->N, a->elem);
   }
   if (q.write_dz || a->dbias) {
-    const Dz d{a->dy, a->ld_dy, a->z, a->ldz, q.write_dz ? (void*)dz.p : nullptr, q.ld_dz, a->dbias ? sums : nullptr, a->M,
+    const Dz d{a->dy, a->ld_dy, a->z, a->ldz, q.write_dz ? (void*)dz.p : nullptr, q.ld_dz, sums, a->dbias, a->M,
                a->N, q.tx, q.stripe, drop};
     const dim3 grid((q.ld_dz / vec_of(a->elem) + (1 << q.tx) - 1) >> q.tx, q.parts);
     if (a->act == GWN_ACT_NONE) dz_kernel<T, GWN_ACT_NONE><<<grid, 256, 0, s>>>(d);
@@ -885,7 +889,7 @@ int bwd(const gwn_linear_bwd_args* a, hipStream_t s) {
     if (a->act == GWN_ACT_SILU) dz_kernel<T, GWN_ACT_SILU><<<grid, 256, 0, s>>>(d);
     GWN_CHECK_LAUNCH();
   }
-  if (a->dbias) {
+  if (a->dbias && q.parts > 1) {
     colsum_kernel<T><<<(a->N + 31) / 32, 1024, 0, s>>>(sums, q.parts, a->N, (T*)a->dbias);
     GWN_CHECK_LAUNCH();
   }

@@ -12,6 +12,9 @@ one element that the program advances once a step (``seed.add_(1)``, also inside
 ``salt`` numbers the mask within the step.  A seed that was advanced between a forward and its
 backward is refused by autograd's version check, since the backward rebuilds the forward's mask.
 
+Forward and backward may be captured into a graph (with autograd's own rule: while one is captured, no
+eager graph that reaches the same leaves may be alive); replays read ``seed`` anew.
+
 The tensors of one call share a device and a type (layer norm's parameters may stay float32); work
 is queued on that device's current stream.  Inputs may be strided over their leading axes; where
 the last axis is not contiguous or the leading axes do not fold into rows, a copy is made.
