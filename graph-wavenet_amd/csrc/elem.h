@@ -26,6 +26,29 @@ __device__ __forceinline__ void store(T* p, const Pack<T, N>& v) {
   *reinterpret_cast<Pack<T, N>*>(p) = v;
 }
 
+// The same where a load's latency counts and rows are of odd lengths: a 16-byte load off a 4-byte border
+// takes more than twice as long, so 16-bit values are loaded by the whole dwords that hold them and
+// shifted into place (12 rows of 1999 by 1030 columns in f16: 13.4 -> 8.5 us; where many rows stream, as in
+// layer norm, the plain load is the faster one).
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_odd(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return load<T, N>(p);
+  } else {
+    const unsigned long long a = (unsigned long long)p;
+    const unsigned sh = (unsigned)(a & 2) * 8;
+    const unsigned* d = (const unsigned*)(a & ~3ull);
+    const Pack<unsigned, N / 2> lo = load<unsigned, N / 2>(d);
+    const unsigned last = d[N / 2 - (sh ? 0 : 1)];  // never a dword without a value
+    Pack<T, N> r;
+    unsigned o[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) o[i] = __builtin_amdgcn_alignbit(i + 1 < N / 2 ? lo.v[i + 1] : last, lo.v[i], sh);
+    __builtin_memcpy(&r, o, sizeof(r));
+    return r;
+  }
+}
+
 // ---- dropout ---------------------------------------------------------------------------------
 // Counter based: element i of a tensor is kept by the mask of (seed, salt) iff u24(i) >= thr, thr =
 // ceil(p 2^24).  The 64-bit key is two rounds of the SplitMix64 finaliser (Steele, Lea and Flood

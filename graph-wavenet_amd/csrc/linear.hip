@@ -494,7 +494,7 @@ __device__ __forceinline__ Pack<T, V> load_end(const T* row, int k, int K) {
   Pack<T, V> a;
   if (K >= V) {
     const int at = k + V <= K ? k : K - V;
-    a = load<T, V>(row + at);
+    a = load_odd<T, V>(row + at);
 #pragma unroll
     for (int j = 0; j < V; ++j) a.v[j] = at + j >= k ? a.v[j] : (T)0.0f;
   } else {
@@ -504,7 +504,7 @@ __device__ __forceinline__ Pack<T, V> load_end(const T* row, int k, int K) {
   return a;
 }
 
-template <typename T, int MT>
+template <typename T, int MT, bool ODD>  // ODD: rows that do not start on 4-byte borders
 __global__ __launch_bounds__(1024) void few_kernel(const Few p) {
   constexpr int V = Vec<T>::N, KS = 4 * V, U = 4, LD = 20;
   __shared__ __attribute__((aligned(16))) float sums[16][16 * MT][LD];
@@ -522,9 +522,10 @@ __global__ __launch_bounds__(1024) void few_kernel(const Few p) {
     if (k0 + KS * U <= p.K) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        a[u] = load<T, V>(w + k0 + u * KS + kl);
+        const int k = k0 + u * KS + kl;
+        a[u] = ODD ? load_odd<T, V>(w + k) : load<T, V>(w + k);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) b[i][u] = load<T, V>(x[i] + k0 + u * KS + kl);
+        for (int i = 0; i < MT; ++i) b[i][u] = ODD ? load_odd<T, V>(x[i] + k) : load<T, V>(x[i] + k);
       }
     } else {
 #pragma unroll
@@ -809,10 +810,11 @@ int fwd(const gwn_linear_args* a, hipStream_t s) {
     const Few p{a->x, a->ldx, a->w, a->ldw, a->M, a->N, a->K, e};
     const int turn = 16 * vec_of(a->elem), turns = (a->K + turn - 1) / turn;  // contraction values a wave takes at once
     const int threads = 64 * (turns < 16 ? turns : 16), grid = (a->N + 15) / 16;
+    const bool odd = sizeof(T) == 2 && (((size_t)a->x | (size_t)a->w | (size_t)(a->ldx * 2) | (size_t)(a->ldw * 2)) & 3);
     if (a->M <= 16)
-      few_kernel<T, 1><<<grid, threads, 0, s>>>(p);
+      (odd ? few_kernel<T, 1, true> : few_kernel<T, 1, false>)<<<grid, threads, 0, s>>>(p);
     else
-      few_kernel<T, 2><<<grid, threads, 0, s>>>(p);
+      (odd ? few_kernel<T, 2, true> : few_kernel<T, 2, false>)<<<grid, threads, 0, s>>>(p);
     GWN_CHECK_LAUNCH();
     return GWN_OK;
   }
