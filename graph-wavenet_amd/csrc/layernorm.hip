@@ -13,6 +13,11 @@
 // registers over all rows its group sees, a workgroup adds its groups up and writes one partial row,
 // and a second launch adds the partial rows in a fixed order.  Rows longer than a workgroup's
 // registers are looped over (they stay in the L2 cache between the passes).
+//
+// Measured, 20800 x 4096 in bf16: forward 67-71 us, backward 98 us + 5 us for the partial rows, 5.0 and 5.2
+// TB/s, as a large copy; 32 to 8192 channels run at 4.6 to 5.2 TB/s, odd widths at 2.5 to 5 (half-empty
+// waves, unaligned pieces), looped rows at 1.8 to 2.6.  Several vectors a lane took the backward's
+// registers and with them the waves that hide its latency: 195 us with two.
 #include "elem.h"
 
 using namespace elem;

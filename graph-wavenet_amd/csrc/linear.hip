@@ -123,9 +123,16 @@ __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int
 // address (swizzle, swizzle_m).  M rows of 16-bit values are read by ds_read_b64_tr_b16, which hands each
 // lane four k of its own column.  What lies outside
 // the matrices is a load past its buffer resource, which gives zeros.
+// Measured (bf16, one launch): 8192^3 842 us = 1306 TFLOP/s (a library product of the same operands
+// 1540), matrix units busy 72-77% of the cycles at the clock that the power limit leaves; 20800 x 2048 x
+// 8192 with gelu and z 737 us = 947 TFLOP/s.  With the loads in one burst behind the barrier and K rows
+// swizzled by row & 7 (half of the LDS cycles conflicts) 8192^3 took 899 us; 64 bytes of k in 4 or 5
+// buffers 920, 128 x 256 tiles two a compute unit 1069, 4 waves of 128 x 128 810 but 10% more with an
+// epilogue; fragment reads between the products, and wave priorities, changed nothing.
 // An operand needs 16-byte aligned rows of whole 16-byte pieces; others are copied to such rows first.
 
 enum { K_ROWS = 0, M_ROWS = 1 };
+constexpr int BB = 128, PIECES = BB / 16, PARTS = BB / 32;  // bytes of k a step, its loads and its parts a row
 constexpr unsigned OOR = 0x7ffffff0u;  // past every resource
 constexpr long MAX_LD = 1 << 20;       // rows further apart are copied: offsets within a tile fit 31 bits
 
@@ -159,32 +166,32 @@ __device__ __forceinline__ void load_lds(u32x4 rs, unsigned off, unsigned lds) {
       : "memory");  // m0 is reserved: the compiler sets it before each use of its own, and has none here
 }
 
-// where in a K row of P pieces piece 0 lies: rows that one LDS cycle reads together (16 of them, 256
-// bytes; lanes 0-3, 12-15, 20-27 and the rest) fall on different banks
-template <int P> __device__ __forceinline__ int swizzle(int row) { return P == 8 ? (row >> 1) & 7 : (row >> 2) & 3; }
+// where in a K row piece 0 lies: the 16 rows that one LDS cycle reads together (256 bytes; lanes 0-3,
+// 12-15, 20-27 and the rest) fall on different banks
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 
 // the same for an M row of 16-bit values, read 4 rows x 32 columns at a time
 template <typename T, int R> __device__ __forceinline__ int swizzle_m(int k) {
   return sizeof(T) == 4 ? 0 : R >= 128 ? (k & 3) << 2 : R == 64 ? (k & 2) << 1 : 0;
 }
 
-// R rows (or columns) of an operand, one step of BB bytes of k, by NT threads
-template <typename T, int L, int R, int NT, int BB>
+// R rows (or columns) of an operand, one step of k, by NT threads
+template <typename T, int L, int R, int NT>
 struct Stage {
-  static constexpr int E = 16 / (int)sizeof(T), BK = BB / (int)sizeof(T), P = BB / 16;
-  static constexpr int PER = R * P / NT, CPR = R * (int)sizeof(T) / 16;
-  static_assert(R * P % NT == 0 && NT / P % 16 == 0, "whole loads");
+  static constexpr int E = 16 / (int)sizeof(T), BK = BB / (int)sizeof(T);
+  static constexpr int PER = R * PIECES / NT, CPR = R * (int)sizeof(T) / 16;
+  static_assert(R * PIECES % NT == 0 && NT / PIECES % 16 == 0, "whole loads");
   unsigned off[PER];
   int k;  // K rows: this thread's k within a step
   __device__ __forceinline__ void init(const Operand& o, int r0, int rows) {
     const int tid = threadIdx.x;
     const unsigned ldb = (unsigned)(o.ld * (long)sizeof(T));
     if (L == K_ROWS) {
-      const int c = (tid % P) ^ swizzle<P>(tid / P);
+      const int c = (tid % PIECES) ^ swizzle(tid / PIECES);
       k = c * E;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int r = i * (NT / P) + tid / P;
+        const int r = i * (NT / PIECES) + tid / PIECES;
         off[i] = r0 + r < rows ? r * ldb + c * 16 : OOR;
       }
     } else {
@@ -225,11 +232,11 @@ struct Stage {
 template <typename T> struct Frag { typedef s16x8 type; };
 template <> struct Frag<float> { typedef f32x4 type; };
 
-template <typename T, int L, int R, int BB>
+template <typename T, int L, int R>
 __device__ __forceinline__ typename Frag<T>::type frag(const char* s, int row0, int ks, int lane) {
   const int row = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
   if constexpr (L == K_ROWS) {
-    return *(const typename Frag<T>::type*)(s + row * BB + ((c ^ swizzle<BB / 16>(lane & 31)) << 4));
+    return *(const typename Frag<T>::type*)(s + row * BB + ((c ^ swizzle(lane & 31)) << 4));
   } else if constexpr (sizeof(T) == 2) {
     const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2);
     const int col = row0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
@@ -271,12 +278,12 @@ __device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& spli
   tm = first + id - tn * rows;
 }
 
-template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN, int BB, int S>
+template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   constexpr int NT = 64 * WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 32, TN = WTN / 32;
-  constexpr int BK = BB / (int)sizeof(T), Q = BB / 32, STAGE = (BM + BN) * BB;
+  constexpr int BK = BB / (int)sizeof(T), STAGE = (BM + BN) * BB;
   constexpr int EW = WTN + 4;  // floats a row of the epilogue's image of one wave's 32 rows
-  constexpr int SMEM = S * STAGE > WGM * WGN * 32 * EW * 4 ? S * STAGE : WGM * WGN * 32 * EW * 4;
+  constexpr int SMEM = 2 * STAGE > WGM * WGN * 32 * EW * 4 ? 2 * STAGE : WGM * WGN * 32 * EW * 4;
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -287,8 +294,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   const int m0 = tm * BM, n0 = tn * BN;
   const int kbeg = split * p.kchunk, kend = p.K - kbeg < p.kchunk ? p.K : kbeg + p.kchunk;
 
-  Stage<T, LA, BM, NT, BB> sa;
-  Stage<T, LB, BN, NT, BB> sb;
+  Stage<T, LA, BM, NT> sa;
+  Stage<T, LB, BN, NT> sb;
   sa.init(p.a, m0, p.M);
   sb.init(p.b, n0, p.N);
 
@@ -315,14 +322,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   auto read = [&](int buf, int ks) {
     const char* A = smem + buf * STAGE;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fa[ks & 1][i] = frag<T, LA, BM, BB>(A, wm * WTM + i * 32, ks, lane);
+    for (int i = 0; i < TM; ++i) fa[ks & 1][i] = frag<T, LA, BM>(A, wm * WTM + i * 32, ks, lane);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fb[ks & 1][j] = frag<T, LB, BN, BB>(A + BM * BB, wn * WTN + j * 32, ks, lane);
+    for (int j = 0; j < TN; ++j) fb[ks & 1][j] = frag<T, LB, BN>(A + BM * BB, wn * WTN + j * 32, ks, lane);
   };
-  // A part's products (32 bytes of k).  The step's loads go between those of its first SPREAD parts:
+  // A part's products (32 bytes of k).  The step's loads go between those of its first two parts:
   // all at once they would keep the wave from its products until the address unit has taken the
   // whole workgroup's, 16 cycles each.
-  constexpr int MM = TM * TN * (sizeof(T) == 2 ? 1 : 4), SPREAD = S == 2 ? Q / 2 : Q;
+  constexpr int MM = TM * TN * (sizeof(T) == 2 ? 1 : 4);
   auto multiply = [&](int ks, int part, int to) {
 #pragma unroll
     for (int q = 0; q < MM; ++q) {
@@ -331,9 +338,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
         acc[i][j] = mma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], T());
       else
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[ks & 1][i][e], fb[ks & 1][j][e], acc[i][j], 0, 0, 0);
-      // loads l with l / LOADS < (part MM + q + 1) / (SPREAD MM)
-      if (part < SPREAD) {
-        const int done = (part * MM + q) * LOADS / (SPREAD * MM), next = (part * MM + q + 1) * LOADS / (SPREAD * MM);
+      // loads l with l / LOADS < (part MM + q + 1) / (2 MM)
+      if (part < 2) {
+        const int done = (part * MM + q) * LOADS / (2 * MM), next = (part * MM + q + 1) * LOADS / (2 * MM);
         if (next > done) {
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -343,45 +350,39 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
       }
     }
   };
-  // S buffers: while one is multiplied the next S - 1 are in flight or landed.  A step's last part is
-  // multiplied behind the barrier that ends it: by then all its fragments are in registers, so its
-  // buffer is free for the loads of the step S - 1 later, and the next step's first fragments arrive
-  // under those products.
+  // Two buffers: while one is multiplied the next step is in flight.  A step's last part is multiplied
+  // behind the barrier that ends it: by then all its fragments are in registers, so its buffer is free
+  // for the loads of the step after next, and the next step's first fragments arrive under those
+  // products.
   auto turn = [&]() {
-    static_assert((S - 2) * LOADS < 16, "vmcnt in one field");
-    __builtin_amdgcn_s_waitcnt(0x0070 | (S - 2) * LOADS);  // vmcnt: all but the last S - 2 steps' loads; lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   if (kbeg < kend) {
+    seek(kbeg);
 #pragma unroll
-    for (int b = 0; b < S - 1; ++b) {
-      seek(kbeg + b * BK);
-#pragma unroll
-      for (int l = 0; l < LOADS; ++l) issue(l, b);
-    }
+    for (int l = 0; l < LOADS; ++l) issue(l, 0);
     turn();
     read(0, 0);
-    seek(kbeg + (S - 1) * BK);
-    int buf = 0, to = S - 1;
+    seek(kbeg + BK);
 #pragma unroll
-    for (int l = 0; l < LOADS / SPREAD; ++l) issue(l, to);
-    for (int k0 = kbeg; k0 < kend; k0 += BK) {
+    for (int l = 0; l < LOADS / 2; ++l) issue(l, 1);
+    int buf = 0;
+    for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
 #pragma unroll
-      for (int ks = 0; ks < Q - 1; ++ks) {
+      for (int ks = 0; ks < PARTS - 1; ++ks) {
         read(buf, ks + 1);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(ks, ks + 1, to);
+        multiply(ks, ks + 1, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       turn();
-      to = buf;
-      buf = buf + 1 == S ? 0 : buf + 1;
-      read(buf, 0);  // past the last step: zeros, not used
-      seek(k0 + S * BK);
+      read(buf ^ 1, 0);  // past the last step: zeros, not used
+      seek(k0 + 2 * BK);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(Q - 1, 0, to);
+      multiply(PARTS - 1, 0, buf);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // the loads past the end write LDS too: vmcnt(0)
@@ -422,8 +423,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   }
 }
 
-// The splits' sums and the epilogue.  256 / TY pieces of 4 columns x TY lanes of splits a workgroup:
-// where there are few outputs their many splits are read side by side.  Fixed order: a lane's splits
+// The splits' sums and the epilogue, bound by reading the sums.  256 / TY pieces of 4 columns x TY lanes of
+// splits a workgroup: where there are few outputs their many splits are read side by side (32 x 224
+// outputs of 226 splits: 33 -> 5 us).  Fixed order: a lane's splits
 // as they come, then the lanes.
 template <typename T, int TY>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int M, int N, Epi e) {
@@ -559,7 +561,7 @@ __global__ __launch_bounds__(1024) void few_kernel(const Few p) {
   }
 }
 
-// rows [rows][ld] -> [rows][ldo] with zeros past `cols`: a 16-byte piece a thread
+// rows [rows][ld] -> [rows][ldo] with zeros past `cols`: a 16-byte piece a thread (bound by memory)
 template <typename T>
 __global__ __launch_bounds__(256) void copy_rows_kernel(const T* x, long ld, long rows, int cols, T* o, int ldo) {
   constexpr int V = Vec<T>::N;
@@ -592,7 +594,9 @@ struct Dz {
 };
 
 // TX pieces of 16 bytes of columns x a stripe of rows a workgroup, 256 / TX rows at a time; each
-// thread sums its columns in fp32 before dz is rounded.  Bound by memory: dy and z read, dz written.
+// thread sums its columns in fp32 before dz is rounded: dz feeds 16-bit products, so it has their type.
+// Bound by memory: dy and z read, dz written (20800 x 8192 in bf16 with gelu: 237 us, 4.3 TB/s; with one
+// row's loads in flight 276).
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
   typedef typename ZType<T>::type Z;
@@ -651,6 +655,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
   }
 }
 
+// the stripes' sums, 32 columns x 32 lanes of stripes a workgroup (4 to 5 us), fixed order
 template <typename T>
 __global__ __launch_bounds__(1024) void colsum_kernel(const float* part, int nparts, int n, T* out) {
   __shared__ float s[32][33];
@@ -739,12 +744,12 @@ long part_floats(int M, int N, int K, int elem) {
 template <typename T, int LA, int LB>
 void launch_tiles(const Gemm& p, int tile, int grid, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (tile == 0) gemm_kernel<T, LA, LB, 256, 256, 2, 4, 128, 2><<<grid, 512, 0, s>>>(p);
-  if (tile == 1) gemm_kernel<T, LA, LB, 128, 128, 2, 2, 128, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 2) gemm_kernel<T, LA, LB, 128, 64, 2, 2, 128, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 3) gemm_kernel<T, LA, LB, 64, 64, 2, 2, 128, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 4) gemm_kernel<T, LA, LB, 128, 32, 4, 1, 128, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 5) gemm_kernel<T, LA, LB, 32, 128, 1, 4, 128, 2><<<grid, 256, 0, s>>>(p);
+    if (tile == 0) gemm_kernel<T, LA, LB, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
+  if (tile == 1) gemm_kernel<T, LA, LB, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 2) gemm_kernel<T, LA, LB, 128, 64, 2, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 3) gemm_kernel<T, LA, LB, 64, 64, 2, 2><<<grid, 256, 0, s>>>(p);
+  if (tile == 4) gemm_kernel<T, LA, LB, 128, 32, 4, 1><<<grid, 256, 0, s>>>(p);
+  if (tile == 5) gemm_kernel<T, LA, LB, 32, 128, 1, 4><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T>
@@ -811,10 +816,9 @@ int fwd(const gwn_linear_args* a, hipStream_t s) {
     const int turn = 16 * vec_of(a->elem), turns = (a->K + turn - 1) / turn;  // contraction values a wave takes at once
     const int threads = 64 * (turns < 16 ? turns : 16), grid = (a->N + 15) / 16;
     const bool odd = sizeof(T) == 2 && (((size_t)a->x | (size_t)a->w | (size_t)(a->ldx * 2) | (size_t)(a->ldw * 2)) & 3);
-    if (a->M <= 16)
-      (odd ? few_kernel<T, 1, true> : few_kernel<T, 1, false>)<<<grid, threads, 0, s>>>(p);
-    else
-      (odd ? few_kernel<T, 2, true> : few_kernel<T, 2, false>)<<<grid, threads, 0, s>>>(p);
+    if constexpr (sizeof(T) == 2)
+      if (odd) (a->M <= 16 ? few_kernel<T, 1, true> : few_kernel<T, 2, true>)<<<grid, threads, 0, s>>>(p);
+    if (!odd) (a->M <= 16 ? few_kernel<T, 1, false> : few_kernel<T, 2, false>)<<<grid, threads, 0, s>>>(p);
     GWN_CHECK_LAUNCH();
     return GWN_OK;
   }
