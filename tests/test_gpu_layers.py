@@ -286,6 +286,17 @@ def test_linear_act_infinities(gpu, t):
         assert torch.isfinite(dx).all() and (dx[0] > 0).all()
 
 
+def test_relu_slope_of_tiny_values(gpu):
+    """A positive pre-activation below f16's smallest step has slope 1, zero and a negative one 0."""
+    from gwn_amd.layers import linear_act
+    x = torch.tensor([[2.0 ** -14], [-2.0 ** -14], [0.0]], device=gpu, dtype=torch.float16, requires_grad=True)
+    w = torch.full((8, 1), 2.0 ** -14, device=gpu, dtype=torch.float16)  # z = +-2^-28, 0
+    b = torch.zeros(8, device=gpu, dtype=torch.float16, requires_grad=True)
+    y = linear_act(x, w, b, act="relu")
+    db, = torch.autograd.grad(y, b, torch.tensor([[1.0], [10.0], [100.0]], device=gpu).half().expand(3, 8).contiguous())
+    assert (db == 1.0).all()
+
+
 @pytest.mark.parametrize("act", ["none", "gelu", "gelu_tanh", "silu"])
 def test_linear_act_gradients_against_differences(gpu, act):
     """Along a direction d, (f(+h) - f(-h)) / 2h of f = sum(y dy): off by h^2 / 6 times the third derivative
@@ -812,6 +823,38 @@ def test_feed_forward_block(gpu, t, tol, p):
     m.eval()
     with torch.no_grad():
         assert torch.equal(m(xd), m(xd, seed=seed))
+
+
+def test_modules(gpu):
+    from gwn_amd.layers import Dropout, LayerNorm, LinearAct, dropout, layer_norm, linear_act
+    x, r = torch.randn(9, 24, device=gpu), torch.randn(9, 24, device=gpu)
+    seed = torch.tensor([6], device=gpu)
+    d = Dropout(0.4, salt=3)
+    assert torch.equal(d(x, seed), dropout(x, 0.4, seed, salt=3))
+    assert torch.equal(d(x, seed, residual=r), dropout(x, 0.4, seed, salt=3, residual=r))
+    with pytest.raises(RuntimeError):
+        d(x)
+    d.eval()
+    assert torch.equal(d(x), x) and torch.equal(d(x, residual=r), x + r)
+    m = LinearAct(24, 24, "silu", 0.4, salt=5).to(gpu)
+    assert torch.equal(m(x, r, seed), linear_act(x, m.weight, m.bias, "silu", r, 0.4, seed, 5))
+    m.eval()
+    assert torch.equal(m(x), linear_act(x, m.weight, m.bias, "silu"))
+    n = LayerNorm(24, eps=1e-3).to(gpu)
+    assert torch.equal(n(x), layer_norm(x, n.weight, n.bias, 1e-3))
+
+
+def test_checkpointed_block(gpu):
+    """Recomputed in the backward, the block draws the same masks: the gradients are the same."""
+    from torch.utils.checkpoint import checkpoint
+    m = feed_forward("f32", gpu, 0.3)
+    x = torch.randn(20, 48, device=gpu, requires_grad=True)
+    seed, dy = torch.tensor([2], device=gpu), torch.randn(20, 48, device=gpu)
+    leaves = [x] + list(m.parameters())
+    want = torch.autograd.grad(m(x, seed=seed), leaves, dy)
+    got = torch.autograd.grad(checkpoint(lambda v: m(v, seed=seed), x, use_reentrant=False), leaves, dy)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
 
 
 def step(m, x, dy, seed):
