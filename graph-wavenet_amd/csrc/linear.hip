@@ -278,12 +278,17 @@ __device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& spli
   tm = first + id - tn * rows;
 }
 
-template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN>
+// ONE: the contraction is one step at most.  Nothing is left to load while it is multiplied, so there is one
+// buffer: up to twice the workgroups fit a compute unit (f32 8 of 128x32; 16-bit 6 of 128x64, where registers
+// do not bind first) and hide each other's loads and stores (158976 x 224 x 32, the
+// best tile of each: bf16 32.5 -> 20.8 us, f32 47.6 -> 40.8; 158976 x 32 x 32: 7.8 -> 5.9 and 12.0 -> 9.7).
+// 256x256 fits once either way and has no such form.
+template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN, bool ONE>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   constexpr int NT = 64 * WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 32, TN = WTN / 32;
   constexpr int BK = BB / (int)sizeof(T), STAGE = (BM + BN) * BB;
   constexpr int EW = WTN + 4;  // floats a row of the epilogue's image of one wave's 32 rows
-  constexpr int SMEM = 2 * STAGE > WGM * WGN * 32 * EW * 4 ? 2 * STAGE : WGM * WGN * 32 * EW * 4;
+  constexpr int BUFS = (ONE ? 1 : 2) * STAGE, IMAGES = WGM * WGN * 32 * EW * 4, SMEM = BUFS > IMAGES ? BUFS : IMAGES;
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -360,7 +365,18 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  if (kbeg < kend) {
+  if (ONE && kbeg < kend) {
+    seek(kbeg);
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) issue(l, 0);
+    turn();
+    read(0, 0);
+#pragma unroll
+    for (int ks = 0; ks < PARTS; ++ks) {
+      if (ks + 1 < PARTS) read(0, ks + 1);
+      multiply(ks, 2, 0);
+    }
+  } else if (kbeg < kend) {
     seek(kbeg);
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) issue(l, 0);
@@ -726,6 +742,11 @@ Shape shape_of(int M, int N, int K, int elem) {
       const double all = c.at_once * step, some = rest * step;
       double time = full * ((all > co.latency ? all : co.latency) * chunk + fixed * co.more);
       if (rest) time += (some > co.latency ? some : co.latency) * chunk + fixed;
+      // A contraction of one step in 16 bits (one buffer, up to twice the workgroups): loads, products and stores follow
+      // each other in each workgroup, and as many as fit hide only their latency.  The tile so chosen is
+      // within 2% of the fastest of 12 measured products, the sum above loses 15% (158976 x 224 x 32, 13248 x
+      // 512 x 64); in f32 the sum above already takes the fastest or one within 1%.
+      if (steps == 1 && !wide) time = share * (step + fixed) * (c.at_once < 3 ? 3.0 / c.at_once : 1.0);
       if (splits > 1) time += co.join + 8.0 * M * N * splits * co.join_byte;
       if (time < least) {
         least = time;
@@ -741,15 +762,22 @@ long part_floats(int M, int N, int K, int elem) {
   return s.splits > 1 ? up((long)s.splits * M * N, 4) : 0;
 }
 
+template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN>
+void launch_tile(const Gemm& p, int grid, hipStream_t s) {
+  if (p.K <= BB / (int)sizeof(T) && BM < 256)
+    gemm_kernel<T, LA, LB, BM, BN, WGM, WGN, BM < 256><<<grid, 64 * WGM * WGN, 0, s>>>(p);
+  else
+    gemm_kernel<T, LA, LB, BM, BN, WGM, WGN, false><<<grid, 64 * WGM * WGN, 0, s>>>(p);
+}
 template <typename T, int LA, int LB>
 void launch_tiles(const Gemm& p, int tile, int grid, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (tile == 0) gemm_kernel<T, LA, LB, 256, 256, 2, 4><<<grid, 512, 0, s>>>(p);
-  if (tile == 1) gemm_kernel<T, LA, LB, 128, 128, 2, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 2) gemm_kernel<T, LA, LB, 128, 64, 2, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 3) gemm_kernel<T, LA, LB, 64, 64, 2, 2><<<grid, 256, 0, s>>>(p);
-  if (tile == 4) gemm_kernel<T, LA, LB, 128, 32, 4, 1><<<grid, 256, 0, s>>>(p);
-  if (tile == 5) gemm_kernel<T, LA, LB, 32, 128, 1, 4><<<grid, 256, 0, s>>>(p);
+    if (tile == 0) launch_tile<T, LA, LB, 256, 256, 2, 4>(p, grid, s);
+  if (tile == 1) launch_tile<T, LA, LB, 128, 128, 2, 2>(p, grid, s);
+  if (tile == 2) launch_tile<T, LA, LB, 128, 64, 2, 2>(p, grid, s);
+  if (tile == 3) launch_tile<T, LA, LB, 64, 64, 2, 2>(p, grid, s);
+  if (tile == 4) launch_tile<T, LA, LB, 128, 32, 4, 1>(p, grid, s);
+  if (tile == 5) launch_tile<T, LA, LB, 32, 128, 1, 4>(p, grid, s);
 }
 
 template <typename T>

@@ -208,6 +208,17 @@ def test_linear_act_larger(gpu, t, m, k, n):
 
 
 @pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("m,k,n", [(9000, 64, 96), (9000, 65, 63), (20000, 24, 40), (12000, 32, 224), (1300, 64, 600),
+                                   (200, 31, 33), (64, 300, 200), (33, 200, 520), (12000, 1, 1)])
+def test_linear_act_short_contractions(gpu, t, m, k, n):
+    """Contractions of one step of the tiles (64 values, 32 in f32), just under and just over it, each
+    tile's width, forward and both gradients."""
+    c = LinearCase(m, k, n, t, "silu", True, True, 0.1)
+    y, got = run_linear(c, gpu)
+    c.check(y=y, **got)
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
 def test_linear_act_strides_and_offsets(gpu, t):
     """x as a column slice that starts off a 16-byte border, a transposed weight, x with swapped
     leading axes, an expanded output gradient."""
