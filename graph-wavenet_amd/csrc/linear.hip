@@ -279,10 +279,9 @@ __device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& spli
 }
 
 // ONE: the contraction is one step at most.  Nothing is left to load while it is multiplied, so there is one
-// buffer: up to twice the workgroups fit a compute unit (f32 8 of 128x32; 16-bit 6 of 128x64, where registers
-// do not bind first) and hide each other's loads and stores (158976 x 224 x 32, the
-// best tile of each: bf16 32.5 -> 20.8 us, f32 47.6 -> 40.8; 158976 x 32 x 32: 7.8 -> 5.9 and 12.0 -> 9.7).
-// 256x256 fits once either way and has no such form.
+// buffer: more workgroups fit a compute unit (f32: 8 of 128x32 for 4; 16-bit: 5 of 128x64 for 3, by their
+// registers) and hide each other's loads and stores.  158976 x 224 x 32, the best tile of each: bf16 32.5 -> 20.8
+// us, f32 47.6 -> 40.8; 158976 x 32 x 32: 7.8 -> 5.9 and 12.0 -> 9.7.  256x256 has no such form: it fits once either way.
 template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN, bool ONE>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   constexpr int NT = 64 * WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 32, TN = WTN / 32;
@@ -742,10 +741,10 @@ Shape shape_of(int M, int N, int K, int elem) {
       const double all = c.at_once * step, some = rest * step;
       double time = full * ((all > co.latency ? all : co.latency) * chunk + fixed * co.more);
       if (rest) time += (some > co.latency ? some : co.latency) * chunk + fixed;
-      // A contraction of one step in 16 bits (one buffer, up to twice the workgroups): loads, products and stores follow
-      // each other in each workgroup, and as many as fit hide only their latency.  The tile so chosen is
-      // within 2% of the fastest of 12 measured products, the sum above loses 15% (158976 x 224 x 32, 13248 x
-      // 512 x 64); in f32 the sum above already takes the fastest or one within 1%.
+      // A contraction of one step in 16 bits (one buffer): loads, products and stores follow each other in each
+      // workgroup, and as many as fit hide only their latency.  Of 12 measured products this takes the fastest
+      // tile or one within 2%, the sum above loses 15% (158976 x 224 x 32, 13248 x 512 x 64); in f32 the
+      // sum above does so by itself.
       if (steps == 1 && !wide) time = share * (step + fixed) * (c.at_once < 3 ? 3.0 / c.at_once : 1.0);
       if (splits > 1) time += co.join + 8.0 * M * N * splits * co.join_byte;
       if (time < least) {
