@@ -71,24 +71,38 @@ __device__ __forceinline__ void store_f(T* p, const float (&v)[V], int rem) {
 template <int V>
 __device__ __forceinline__ void drop_vec(float (&v)[V], DropKey& key, const Drop& d, unsigned long long i) {
   key.seek(i);
-  const bool steps = (unsigned)i > 0xFFFFFFFFu - V;  // the high half steps within
+  bool keep[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (steps) key.seek(i + j);
-    v[j] = key.keep((unsigned)i + j, d.thr) ? v[j] * d.scale : 0.0f;
+  for (int j = 0; j < V; ++j) keep[j] = key.keep((unsigned)i + j, d.thr);
+  if ((unsigned)i > 0xFFFFFFFFu - V) {  // the high half steps within
+    const unsigned first = (unsigned)i;
+    key.rekey(key.hi + 1);
+#pragma unroll
+    for (int j = 1; j < V; ++j)
+      if (first + j < first) keep[j] = key.keep(first + j, d.thr);
   }
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = keep[j] ? v[j] * d.scale : 0.0f;
 }
 
-// V columns n .. of row m, of which `rem` lie within N
 template <typename T, int V>
-__device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int n, int rem, float (&v)[V]) {
-  typedef typename ZType<T>::type Z;
-  if (e.bias) {
-    float b[V];
-    load_f<T, V>(b, (const T*)e.bias + n, rem);
+__device__ __forceinline__ Pack<T, V> load_part(const T* p, int rem) {
+  if (rem >= V) return load<T, V>(p);
+  Pack<T, V> a;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] += b[j];
-  }
+  for (int j = 0; j < V; ++j) a.v[j] = j < rem ? p[j] : (T)0.0f;
+  return a;
+}
+
+// V columns n .. of row m, of which `rem` lie within N: all of the epilogue before the residual; b is the
+// bias's piece
+template <typename T, int V>
+__device__ __forceinline__ void before_residual(const Epi& e, DropKey& key, long m, int n, int rem, float (&v)[V],
+                                                const Pack<T, V>& b) {
+  typedef typename ZType<T>::type Z;
+  if (e.bias)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += (float)b.v[j];
   if (e.z) {
     Z* z = (Z*)e.z + m * e.ldz + n;
     Pack<Z, V> a;
@@ -104,14 +118,20 @@ __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int
   }
   act_vec<is16<T>, V>(v, e.act);
   if (e.drop.thr) drop_vec<V>(v, key, e.drop, (unsigned long long)m * e.N + n);
-  if (e.res) {
-    float r[V];
-    load_f<T, V>(r, (const T*)e.res + m * e.ld_res + n, rem);
+}
+template <typename T, int V>
+__device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int n, int rem, float (&v)[V]) {
+  Pack<T, V> b, r;
+  if (e.bias) b = load_part<T, V>((const T*)e.bias + n, rem);
+  if (e.res) r = load_part<T, V>((const T*)e.res + m * e.ld_res + n, rem);
+  before_residual<T, V>(e, key, m, n, rem, v, b);
+  if (e.res)
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] += r[j];
-  }
+    for (int j = 0; j < V; ++j) v[j] += (float)r.v[j];
   store_f<T, V>((T*)e.y + m * e.ldy + n, v, rem);
 }
+
+template <int I> struct Int { static constexpr int value = I; };
 
 // ---- the tile kernel ------------------------------------------------------------------------------
 //
@@ -403,35 +423,76 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // the loads past the end write LDS too: vmcnt(0)
   }
 
-  // 32 rows of a wave at a time through LDS, from the accumulators' layout to whole row pieces
+  // 32 rows of a wave at a time through LDS, from the accumulators' layout to whole row pieces.  A wait for
+  // a load is a wait for all stores before it too, so the bias is read once, and a piece's residual of the
+  // next 32 rows before this one's are stored; blocks at the edges read both as they go.  20800 x 2048 ->
+  // 8192 in f16: 666 -> 641 us with a bias, 829 -> 673 with a residual too, 991 -> 846 with gelu, dropout and z.
+  // Four blocks share their code (unrolled it runs cold through the instruction cache: 720 us with a
+  // bias); two are unrolled (158976 x 32 -> 224: 28 -> 22 us).
+  constexpr int V = 16 / (int)sizeof(T), LPR = WTN / V, RPI = 64 / LPR, PIECES = 32 / RPI;
+  constexpr int ROLL = TM == 4 ? 1 : TM;
+  const int n = n0 + wn * WTN + (lane % LPR) * V, rem = p.N - n, mw = m0 + wm * WTM;
+  const bool inside = p.splits == 1 && n0 + (wn + 1) * WTN <= p.N;
+  Pack<T, V> bias, res[PIECES];
+  auto fetch = [&](int q, int row) {
+    res[q] = load<T, V>((const T*)p.e.res + (long)(row + q * RPI + lane / LPR) * p.e.ld_res + n);
+  };
+  if (inside && p.e.bias) bias = load<T, V>((const T*)p.e.bias + n);
+  if (inside && p.e.res && mw + 32 <= p.M)
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) fetch(q, mw);
   __syncthreads();
-  constexpr int V = 16 / (int)sizeof(T), LPR = WTN / V, RPI = 64 / LPR;
   float* img = (float*)smem + wave * 32 * EW;
   DropKey key;
   if (p.e.drop.thr) key.init(p.e.drop, (unsigned long long)m0 * p.N + n0);
-  const int n = n0 + wn * WTN + (lane % LPR) * V, rem = p.N - n;
-#pragma unroll
+#pragma unroll ROLL
   for (int i = 0; i < TM; ++i) {
+    const int mi = mw + i * 32;
+    auto image = [&](auto I) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          img[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * EW + j * 32 + (lane & 31)] = acc[decltype(I)::value][j][r];
+    };
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        img[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * EW + j * 32 + (lane & 31)] = acc[i][j][r];
+    static_assert(TM == 1 || TM == 2 || TM == 4, "blocks");
+    if (TM == 1 || i == 0) image(Int<0>());
+    if (TM > 1 && i == 1) image(Int<1 % TM>());
+    if (TM > 2 && i == 2) image(Int<2 % TM>());
+    if (TM > 2 && i == 3) image(Int<3 % TM>());
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-    for (int q = 0; q < 32 / RPI; ++q) {
-      const int row = q * RPI + lane / LPR;
-      const long m = m0 + wm * WTM + i * 32 + row;
-      float v[V];
+    auto piece = [&](int q, float (&v)[V]) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = img[row * EW + (lane % LPR) * V + j];
-      if (m < p.M && rem > 0) {
-        if (p.splits > 1)
-          store_f<float, V>(p.part + ((long)split * p.M + m) * p.N + n, v, rem);
-        else
-          epilogue<T, V>(p.e, key, m, n, rem, v);
+      for (int j = 0; j < V; ++j) v[j] = img[(q * RPI + lane / LPR) * EW + (lane % LPR) * V + j];
+    };
+    if (inside && mi + 32 <= p.M) {
+      const int next = i + 1 < TM && mi + 64 <= p.M ? mi + 32 : mi;  // these rows again where none follow
+#pragma unroll
+      for (int q = 0; q < PIECES; ++q) {
+        float v[V];
+        piece(q, v);
+        before_residual<T, V>(p.e, key, mi + q * RPI + lane / LPR, n, V, v, bias);
+        if (p.e.res) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] += (float)res[q].v[j];
+          if (TM == 4 || i + 1 < TM) fetch(q, next);
+        }
+        store_f<T, V>((T*)p.e.y + (long)(mi + q * RPI + lane / LPR) * p.e.ldy + n, v, V);
+      }
+    } else {
+#pragma unroll 1
+      for (int q = 0; q < PIECES; ++q) {
+        const long m = mi + q * RPI + lane / LPR;
+        float v[V];
+        piece(q, v);
+        if (m < p.M && rem > 0) {
+          if (p.splits > 1)
+            store_f<float, V>(p.part + ((long)split * p.M + m) * p.N + n, v, rem);
+          else
+            epilogue<T, V>(p.e, key, m, n, rem, v);
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
