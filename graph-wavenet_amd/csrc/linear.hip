@@ -67,6 +67,9 @@ __device__ __forceinline__ void store_f(T* p, const float (&v)[V], int rem) {
   }
 }
 
+// an epilogue that computes
+bool full(const Epi& e) { return e.act != GWN_ACT_NONE || e.drop.thr; }
+
 // the mask on elements i .. i + V - 1
 template <int V>
 __device__ __forceinline__ void drop_vec(float (&v)[V], DropKey& key, const Drop& d, unsigned long long i) {
@@ -301,7 +304,7 @@ __device__ __forceinline__ void place(const Gemm& p, int& tm, int& tn, int& spli
 // ONE: the contraction is one step at most.  Nothing is left to load while it is multiplied, so there is one
 // buffer: more workgroups fit a compute unit (f32: 8 of 128x32 for 4; 16-bit: 5 of 128x64 for 3, by their
 // registers) and hide each other's loads and stores.  158976 x 224 x 32, the best tile of each: bf16 32.5 -> 20.8
-// us, f32 47.6 -> 40.8; 158976 x 32 x 32: 7.8 -> 5.9 and 12.0 -> 9.7.  256x256 has no such form: it fits once either way.
+// us, f32 47.6 -> 40.8; 158976 x 32 x 32: 7.8 -> 5.9 and 12.0 -> 9.7.  256x256 fits once either way: no such form.
 template <typename T, int LA, int LB, int BM, int BN, int WGM, int WGN, bool ONE>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   constexpr int NT = 64 * WGM * WGN, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 32, TN = WTN / 32;
@@ -813,12 +816,15 @@ long copy_floats(long rows, int cols, int elem) { return up(rows * up(cols, vec_
 struct Tile { int bm, bn, at_once; double rate16, rate32; };  // rates: shares of 4096, 256 operations a cycle
 constexpr Tile TILES[] = {{256, 256, 1, 0.66, 0.0}, {128, 128, 2, 0.62, 0.86}, {128, 64, 3, 0.30, 0.88},
                           {64, 64, 5, 0.33, 0.88},  {128, 32, 4, 0.17, 0.82},  {32, 128, 4, 0.24, 0.85}};
-struct Cost { double load, latency, fixed, epilogue, more, join, join_byte; };
-constexpr Cost COST16 = {1.0 / 26, 2300, 200, 0.16, 1.6, 16000, 1.0 / 710};
-constexpr Cost COST32 = {0, 1400, 0, 0, 1, 3200, 1.0 / 1800};
+struct Cost { double load, latency, fixed, epilogue, full, more, join, join_byte; };
+constexpr Cost COST16 = {1.0 / 26, 2300, 200, 0.16, 0.28, 1.6, 16000, 1.0 / 710};
+constexpr Cost COST32 = {0, 1400, 0, 0, 0, 1, 3200, 1.0 / 1800};
 struct Shape { int tile, tiles_m, tiles_n, splits, kchunk; };
 
-Shape shape_of(int M, int N, int K, int elem) {
+// full_epilogue: with an activation or dropout (a residual's loads hide in any tile).  Weighed as one without, 7
+// products in 16 bits are 4 to 6% slower than with the fastest tile on average, 17% at worst; so 2 to 4% and 10%
+// (5200 x 512 x 2048 with everything: 39.2 -> 37.1 us).  In f32 the products outlast it.
+Shape shape_of(int M, int N, int K, int elem, bool full_epilogue) {
   const bool wide = elem == GWN_ELEM_F32;
   const Cost& co = wide ? COST32 : COST16;
   const int bk = wide ? 32 : 64;
@@ -831,7 +837,8 @@ Shape shape_of(int M, int N, int K, int elem) {
     if (rate == 0) continue;
     const long tm = (M + c.bm - 1) / c.bm, tn = (N + c.bn - 1) / c.bn, tiles = tm * tn;
     const double product = 2.0 * c.bm * c.bn * bk / rate, loads = (c.bm + c.bn) * 128 * co.load;
-    const double step = product > loads ? product : loads, fixed = co.fixed + c.bm * c.bn * co.epilogue;
+    const double step = product > loads ? product : loads;
+    const double fixed = co.fixed + c.bm * c.bn * (full_epilogue ? co.full : co.epilogue);
     long last = 0;
     for (long want = 1; want <= 512; want += (want + 3) / 4) {
       const long chunk = (steps + want - 1) / want, splits = chunk ? (steps + chunk - 1) / chunk : 1;
@@ -856,8 +863,8 @@ Shape shape_of(int M, int N, int K, int elem) {
   }
   return best;
 }
-long part_floats(int M, int N, int K, int elem) {
-  const Shape s = shape_of(M, N, K, elem);
+long part_floats(int M, int N, int K, int elem, bool full_epilogue = false) {
+  const Shape s = shape_of(M, N, K, elem, full_epilogue);
   return s.splits > 1 ? up((long)s.splits * M * N, 4) : 0;
 }
 
@@ -882,7 +889,7 @@ void launch_tiles(const Gemm& p, int tile, int grid, hipStream_t s) {
 template <typename T>
 int gemm(int la, int lb, Operand a, Operand b, int M, int N, int K, int krows, int elem, const Epi& e, float* part,
          hipStream_t s) {
-  const Shape sh = shape_of(M, N, K, elem);
+  const Shape sh = shape_of(M, N, K, elem, full(e));
   const long grid = (long)sh.tiles_m * sh.tiles_n * sh.splits;
   GWN_REQUIRE(grid < (1L << 22), "linear: too many tiles for one launch");
   const Gemm p{a, b, M, N, K, krows, sh.tiles_m, sh.tiles_n, sh.splits, sh.kchunk, part, e};
@@ -926,9 +933,14 @@ bool few_rows(const gwn_linear_args* a) {
   return a->M <= 32 && (long)a->M * a->N <= 131072 && a->K <= (a->M <= 16 ? 4096 : 1024);
 }
 
+Epi epi_of(const gwn_linear_args* a) {
+  return {a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->y, a->ldy, a->N, a->act,
+          drop_of(a->seed_ptr, a->salt, a->drop_p)};
+}
+
 long fwd_floats(const gwn_linear_args* a) {
   if (few_rows(a)) return 0;
-  long f = part_floats(a->M, a->N, a->K, a->elem);
+  long f = part_floats(a->M, a->N, (int)up(a->K, vec_of(a->elem)), a->elem, full(epi_of(a)));
   if (!stageable(a->x, a->ldx, a->K, a->elem)) f += copy_floats(a->M, a->K, a->elem);
   if (!stageable(a->w, a->ldw, a->K, a->elem)) f += copy_floats(a->N, a->K, a->elem);
   return f;
@@ -936,13 +948,13 @@ long fwd_floats(const gwn_linear_args* a) {
 
 template <typename T>
 int fwd(const gwn_linear_args* a, hipStream_t s) {
-  const Epi e{a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->y, a->ldy, a->N, a->act,
-              drop_of(a->seed_ptr, a->salt, a->drop_p)};
+  const Epi e = epi_of(a);
   if (few_rows(a)) {
     const Few p{a->x, a->ldx, a->w, a->ldw, a->M, a->N, a->K, e};
-    const int turn = 16 * vec_of(a->elem), turns = (a->K + turn - 1) / turn;  // contraction values a wave takes at once
+    const int turn = 16 * vec_of(a->elem), turns = (a->K + turn - 1) / turn;  // values a wave takes at once
     const int threads = 64 * (turns < 16 ? turns : 16), grid = (a->N + 15) / 16;
-    const bool odd = sizeof(T) == 2 && (((size_t)a->x | (size_t)a->w | (size_t)(a->ldx * 2) | (size_t)(a->ldw * 2)) & 3);
+    const bool odd =
+        sizeof(T) == 2 && (((size_t)a->x | (size_t)a->w | (size_t)(a->ldx * 2) | (size_t)(a->ldw * 2)) & 3);
     if constexpr (sizeof(T) == 2)
       if (odd) (a->M <= 16 ? few_kernel<T, 1, true> : few_kernel<T, 2, true>)<<<grid, threads, 0, s>>>(p);
     if (!odd) (a->M <= 16 ? few_kernel<T, 1, false> : few_kernel<T, 2, false>)<<<grid, threads, 0, s>>>(p);
