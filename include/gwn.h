@@ -799,7 +799,8 @@ long gwn_layernorm_bwd_workspace_floats(long rows, int c, int elem);
 /* y = residual + D(act(z)), z = x w^T + bias: x [M][ldx] (K values a row), w [N][ldw], bias [N] or
  * NULL, residual [M][ld_res] or NULL, y [M][ldy]; D is gwn_dropout's mask on element m N + n (drop_p
  * 0 = none, seed_ptr unused).  z [M][ldz] (NULL = no backward follows, or act NONE): the pre-activation
- * for the backward, float for f32 elements and otherwise f16, saturated, with its sign kept. */
+ * for the backward, float for f32 elements and otherwise f16 (past its range an infinity; with relu a
+ * positive value stays one).  y may be residual (same ld). */
 typedef struct gwn_linear_args {
   const void* x; long ldx;
   const void* w; long ldw;

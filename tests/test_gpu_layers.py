@@ -671,6 +671,25 @@ def test_linear_entries_leave_the_rest(gpu, t, m, k, n):
 
 
 @pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("m,k,n", [(7, 50, 36), (40, 2000, 24), (500, 40, 300), (999, 300, 67), (4070, 512, 4050)])
+def test_linear_entry_in_place(gpu, t, m, k, n):
+    """y in the residual's memory, with few rows, with the contraction split, and over whole and cut tiles."""
+    import ctypes
+    from gwn_amd import _lib
+    lib, elem = _lib.load(), {"f32": 0, "f16": 1, "bf16": 2}[t]
+    c = LinearCase(m, k, n, t, "silu", True, True, 0.3)
+    x, w, b, y = (v.to(gpu) for v in (c.x, c.w, c.b, c.r))
+    seed = torch.tensor([c.seed], device=gpu)
+    f = _lib.LinearArgs(x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), y.data_ptr(), n, y.data_ptr(), n, None, n, m, n, k,
+                        elem, 4, seed.data_ptr(), c.salt, 0.3, None)
+    ws = torch.full((max(1, lib.gwn_linear_fwd_workspace_floats(ctypes.byref(f))),), math.nan, device=gpu)
+    f.workspace = ws.data_ptr()
+    _lib.check(lib.gwn_linear_fwd(ctypes.byref(f), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    c.check(y=y)
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
 @pytest.mark.parametrize("c", [6, 33, 600, 9000, 40000])
 def test_norm_entries_in_place(gpu, t, c):
     """y over x and dx over dy, rows apart, what lies between them as it was."""
