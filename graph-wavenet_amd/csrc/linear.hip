@@ -40,6 +40,7 @@ struct Epi {
   void* y; long ldy;
   int N, act;
   Drop drop;
+  unsigned long long first;  // position of row 0's first element in the mask
 };
 
 template <typename T, int V>
@@ -120,7 +121,7 @@ __device__ __forceinline__ void before_residual(const Epi& e, DropKey& key, long
     }
   }
   act_vec<is16<T>, V>(v, e.act);
-  if (e.drop.thr) drop_vec<V>(v, key, e.drop, (unsigned long long)m * e.N + n);
+  if (e.drop.thr) drop_vec<V>(v, key, e.drop, e.first + (unsigned long long)m * e.N + n);
 }
 template <typename T, int V>
 __device__ __forceinline__ void epilogue(const Epi& e, DropKey& key, long m, int n, int rem, float (&v)[V]) {
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_kernel(const Gemm p) {
   __syncthreads();
   float* img = (float*)smem + wave * 32 * EW;
   DropKey key;
-  if (p.e.drop.thr) key.init(p.e.drop, (unsigned long long)m0 * p.N + n0);
+  if (p.e.drop.thr) key.init(p.e.drop, p.e.first + (unsigned long long)m0 * p.N + n0);
 #pragma unroll ROLL
   for (int i = 0; i < TM; ++i) {
     const int mi = mw + i * 32;
@@ -886,20 +887,34 @@ void launch_tiles(const Gemm& p, int tile, int grid, hipStream_t s) {
   if (tile == 5) launch_tile<T, LA, LB, 32, 128, 1, 4>(p, grid, s);
 }
 
+// Rows of the result beyond a launch's MOST_TILES go in launches of their own: 2^29 rows of up to 32 columns and
+// more.  (Half of what a grid of 512 threads a workgroup may hold, and place() counts tiles in 32 bits.)
+constexpr long MOST_TILES = 1L << 22;
+
 template <typename T>
-int gemm(int la, int lb, Operand a, Operand b, int M, int N, int K, int krows, int elem, const Epi& e, float* part,
+int gemm(int la, int lb, Operand a, Operand b, int M, int N, int K, int krows, int elem, Epi e, float* part,
          hipStream_t s) {
   const Shape sh = shape_of(M, N, K, elem, full(e));
-  const long grid = (long)sh.tiles_m * sh.tiles_n * sh.splits;
-  GWN_REQUIRE(grid < (1L << 22), "linear: too many tiles for one launch");
-  const Gemm p{a, b, M, N, K, krows, sh.tiles_m, sh.tiles_n, sh.splits, sh.kchunk, part, e};
-  if (la == K_ROWS && lb == K_ROWS)
-    launch_tiles<T, K_ROWS, K_ROWS>(p, sh.tile, (int)grid, s);
-  else if (la == K_ROWS)
-    launch_tiles<T, K_ROWS, M_ROWS>(p, sh.tile, (int)grid, s);
-  else
-    launch_tiles<T, M_ROWS, M_ROWS>(p, sh.tile, (int)grid, s);
-  GWN_CHECK_LAUNCH();
+  const long most = MOST_TILES / sh.tiles_n;  // tiles_n is at most 2^15; splits only where tiles are few
+  for (long t = 0; t < sh.tiles_m; t += most) {
+    const int tm = (int)(sh.tiles_m - t < most ? sh.tiles_m - t : most);
+    const long r0 = t * TILES[sh.tile].bm, rows = t + most < sh.tiles_m ? most * TILES[sh.tile].bm : M - r0;
+    const Operand at{(const T*)a.p + r0 * (la == K_ROWS ? a.ld : 1), a.ld};
+    Epi et = e;
+    et.y = (T*)e.y + r0 * e.ldy;
+    if (e.res) et.res = (const T*)e.res + r0 * e.ld_res;
+    if (e.z) et.z = (typename ZType<T>::type*)e.z + r0 * e.ldz;
+    et.first = (unsigned long long)r0 * e.N;
+    const Gemm p{at, b, (int)rows, N, K, krows, tm, sh.tiles_n, sh.splits, sh.kchunk, part, et};
+    const int grid = tm * sh.tiles_n * sh.splits;
+    if (la == K_ROWS && lb == K_ROWS)
+      launch_tiles<T, K_ROWS, K_ROWS>(p, sh.tile, grid, s);
+    else if (la == K_ROWS)
+      launch_tiles<T, K_ROWS, M_ROWS>(p, sh.tile, grid, s);
+    else
+      launch_tiles<T, M_ROWS, M_ROWS>(p, sh.tile, grid, s);
+    GWN_CHECK_LAUNCH();
+  }
   if (sh.splits > 1) {
     const long pieces = (long)M * ((N + 3) / 4), cus = gwn_device_cus(), most = cus * 16;
     if (pieces >= cus * 256 || sh.splits < 8) {
@@ -935,7 +950,7 @@ bool few_rows(const gwn_linear_args* a) {
 
 Epi epi_of(const gwn_linear_args* a) {
   return {a->bias, a->residual, a->ld_res, a->act == GWN_ACT_NONE ? nullptr : a->z, a->ldz, a->y, a->ldy, a->N, a->act,
-          drop_of(a->seed_ptr, a->salt, a->drop_p)};
+          drop_of(a->seed_ptr, a->salt, a->drop_p), 0};
 }
 
 long fwd_floats(const gwn_linear_args* a) {

@@ -1,0 +1,40 @@
+"""Position-wise layers (``gwn_amd.layers``) at the ends of their ranges: the most rows and channels,
+values near the types' ends, an activation's tail, long sums.  Oracles and bounds are those of
+``test_gpu_layers``."""
+import pytest
+import torch
+
+from test_gpu_layers import E32, F64, LinearCase, TINY, half_step, mask, within
+
+pytestmark = pytest.mark.gpu
+
+
+def test_linear_act_most_rows(gpu):
+    """More rows than one launch's tiles cover (2^22 of at most 128 rows where the result is narrow): values, mask
+    and gradients on both sides of row 2^29 and at the ends are those of the formula at these rows."""
+    from gwn_amd.layers import linear_act
+    m, k, n = 2 ** 29 + 5000, 8, 8
+    c = LinearCase(120, k, n, "bf16", "relu", True, False, 0.5)
+    at = torch.cat([torch.arange(40), torch.arange(2 ** 29 - 20, 2 ** 29 + 20), torch.arange(m - 40, m)]).to(gpu)
+    x = torch.zeros(m, k, device=gpu, dtype=torch.bfloat16)
+    x[at] = c.x.to(gpu)
+    x.requires_grad_()
+    w, b = c.w.to(gpu).requires_grad_(), c.b.to(gpu).requires_grad_()
+    seed = torch.tensor([c.seed], device=gpu)
+    y = linear_act(x, w, b, act="relu", p=0.5, seed=seed, salt=c.salt)
+    keep = torch.cat([mask(c.seed, c.salt, (40, n), 0.5, int(r) * n) for r in (0, 2 ** 29 - 20, m - 40)])
+    z = c.x.double() @ c.w.double().T + c.b.double()  # exact: on grids
+    want = torch.where(keep, z.clamp(min=0) * 2, torch.zeros((), dtype=F64))
+    assert torch.equal(y[at].cpu(), want.to(torch.bfloat16))
+    dy = torch.zeros_like(y)
+    dy[at] = c.dy.to(gpu)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    del y, dy
+    dz = torch.where(keep & (z > 0), c.dy.double() * 2, torch.zeros((), dtype=F64))  # exact in bfloat16
+    u, tiny = half_step("bf16"), TINY["bf16"]
+    for name, got, want, size in (("dx", dx[at], dz @ c.w.double(), dz.abs() @ c.w.double().abs()),
+                                  ("dw", dw, dz.T @ c.x.double(), dz.T.abs() @ c.x.double().abs()),
+                                  ("db", db, dz.sum(0), dz.abs().sum(0))):  # 120 terms, the others are zeros
+        within(name, got, want, 122 * E32 * size + u * want.abs() * (1 + 2.0 ** -8) + tiny)
+    dx[at] = 0
+    assert not dx.any()
