@@ -478,27 +478,32 @@ __global__ __launch_bounds__(THREADS) void ln_cols_long_kernel(const LnBwd p) {
   }
 }
 
-// out[k] = sum over parts of part[.][k]: 32 columns x 32 lanes of parts a workgroup, fixed order
+// out[k] = sum over parts of part[.][k]: 32 columns x 32 lanes of parts a workgroup, fixed order.  The
+// workgroups walk the columns: a grid has fewer than 2^32 threads, and columns go up to 2^31.
+constexpr long REDUCE_GRID = 1 << 16;
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* part, int nparts, int c, W* dgamma, W* dbeta) {
   __shared__ float s[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long k = (long)blockIdx.x * 32 + tx;
-  float v = 0.0f;
-  if (k < 2L * c)
+  for (long first = (long)blockIdx.x * 32; first < 2L * c; first += (long)gridDim.x * 32) {
+    const long k = first + tx;
+    float v = 0.0f;
+    if (k < 2L * c)
 #pragma unroll 8
-    for (int q = ty; q < nparts; q += 32) v += part[(long)q * 2 * c + k];
-  s[ty][tx] = v;
-  __syncthreads();
-  if (ty == 0 && k < 2L * c) {
-    v = 0.0f;
+      for (int q = ty; q < nparts; q += 32) v += part[(long)q * 2 * c + k];
+    s[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && k < 2L * c) {
+      v = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 32; ++q) v += s[q][tx];
-    if (k < c) {
-      if (dgamma) dgamma[k] = (W)v;
-    } else if (dbeta) {
-      dbeta[k - c] = (W)v;
+      for (int q = 0; q < 32; ++q) v += s[q][tx];
+      if (k < c) {
+        if (dgamma) dgamma[k] = (W)v;
+      } else if (dbeta) {
+        dbeta[k - c] = (W)v;
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -577,8 +582,9 @@ int bwd(const LnBwd& p, int elem, void* dgamma, void* dbeta, hipStream_t s) {
     }
   }
   if (!p.part) return GWN_OK;
-  ln_reduce_kernel<W><<<(int)((2L * p.c + 31) / 32), 1024, 0, s>>>(p.part, p.rows ? grid : 0, p.c, (W*)dgamma,
-                                                                   (W*)dbeta);
+  const long blocks = (2L * p.c + 31) / 32;
+  ln_reduce_kernel<W><<<(int)(blocks < REDUCE_GRID ? blocks : REDUCE_GRID), 1024, 0, s>>>(
+      p.part, p.rows ? grid : 0, p.c, (W*)dgamma, (W*)dbeta);
   GWN_CHECK_LAUNCH();
   return GWN_OK;
 }

@@ -38,3 +38,27 @@ def test_linear_act_most_rows(gpu):
         within(name, got, want, 122 * E32 * size + u * want.abs() * (1 + 2.0 ** -8) + tiny)
     dx[at] = 0
     assert not dx.any()
+
+
+def test_layer_norm_many_channels(gpu):
+    """A row of more than 2^26 channels: its parameters' gradients are one term each.  Its values are +-1 in turn, so
+    its statistics are exact but for 8 roundings of fp32."""
+    from gwn_amd.layers import layer_norm
+    c, t = 2 ** 26 + 40, torch.bfloat16
+    x = torch.ones(1, c, device=gpu, dtype=t)
+    x[:, 1::2] = -1
+    w, b = torch.ones(c, device=gpu, dtype=t), torch.full((c,), 0.25, device=gpu, dtype=t)
+    w[c // 3:] = 0.5
+    dy = torch.randn(1, c, device=gpu, generator=torch.Generator(device=gpu).manual_seed(2)).to(t)
+    for v in (x, w, b):
+        v.requires_grad_()
+    y = layer_norm(x, w, b)
+    dw, db = torch.autograd.grad(y, (w, b), dy, retain_graph=True)
+    xh = x.detach().double() * (1 + 1e-5) ** -0.5
+    off = 8 * E32 + half_step("bf16") * (1 + 2.0 ** -8)
+    for at in (slice(0, 4096), slice(c // 3 - 100, c // 3 + 100), slice(2 ** 25 - 64, 2 ** 25 + 64), slice(c - 4096, c)):
+        want = xh[0, at] * w[at].double() + b[at].double()
+        within("y", y[0, at], want.detach().cpu(), (off * want.abs()).detach().cpu())
+        want = dy[0, at].double() * xh[0, at]
+        within("dw", dw[at], want.cpu(), (off * want.abs()).cpu() + TINY["bf16"])
+        assert torch.equal(db[at], dy[0, at])
