@@ -118,6 +118,8 @@ struct Span {
     return TINY && c < V ? j < c : j >= whole(i) - at(i);
   }
   __device__ __forceinline__ bool counts(int i, int j) const { return in(i) && own(i, j); }
+  // whether value j of vector i is one of the row's, this lane's or not
+  __device__ __forceinline__ bool there(int i, int j) const { return in(i) && !(TINY && c < V && j >= c); }
   // zeros where there is no vector
   template <typename T> __device__ __forceinline__ Pack<T, V> get(const T* row, int i) const {
     Pack<T, V> a{};
@@ -317,7 +319,8 @@ __global__ __launch_bounds__(G ? THREADS : I == 1 ? MOST : MOST / 2) void ln_bwd
     for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] = ((float)nx[i].v[j] - mean) * rstd;
+        // 0 where there is none: mean rstd may pass fp32's range, and an infinity by h = 0 is a NaN in the sums
+        v[i][j] = ((float)nx[i].v[j] - mean) * (sp.there(i, j) ? rstd : 0.0f);
         h[i][j] = (float)ny[i].v[j];
       }
     if (row + step < p.rows) fetch(row + step);

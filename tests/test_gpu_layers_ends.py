@@ -4,7 +4,7 @@ values near the types' ends, an activation's tail, long sums.  Oracles and bound
 import pytest
 import torch
 
-from test_gpu_layers import E32, F64, LinearCase, TINY, half_step, mask, within
+from test_gpu_layers import E32, F64, LinearCase, TINY, TYPES, half_step, mask, within
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,27 @@ def test_layer_norm_many_channels(gpu):
         want = dy[0, at].double() * xh[0, at]
         within("dw", dw[at], want.cpu(), (off * want.abs()).cpu() + TINY["bf16"])
         assert torch.equal(db[at], dy[0, at])
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("c", [3, 5, 33, 100, 700, 2052, 20000])
+def test_layer_norm_backward_of_large_constant_rows(gpu, c, t):
+    """Rows of one large value each (a power of two: their sums are exact), a small eps: mean rstd passes fp32's range,
+    but xh = 0 and dx = rstd (h - mean(h)).  A mean of h is off by `chain` additions' roundings."""
+    from gwn_amd.layers import layer_norm
+    eps, dt = 2.0 ** -40, TYPES[t]
+    x = (torch.ones(6, c) * 2.0 ** torch.tensor([110.0, 0.0, -3.0, 108.0, 111.0, 112.0])[:, None]).to(dt)
+    x[2] = -x[4]
+    g = torch.Generator().manual_seed(c)
+    w, b, dy = (1 + 0.2 * torch.randn(c, generator=g)).to(dt), torch.randn(c, generator=g).to(dt), torch.randn(6, c, generator=g).to(dt)
+    leaves = [v.to(gpu).requires_grad_() for v in (x, w, b)]
+    y = layer_norm(*leaves, eps=eps)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.to(gpu))
+    assert torch.equal(y.cpu(), b.expand(6, c)) and not dw.any()
+    h = dy.to(F64) * w.to(F64)
+    chain = 8 * max(8, -(-c // 2048)) + 16
+    rs, mean = 2.0 ** 20, h.mean(1, keepdim=True)
+    want = rs * (h - mean)
+    e = rs * (4 * E32 * (h.abs() + mean.abs()) + (chain + 2) * E32 * h.abs().mean(1, keepdim=True))
+    within("dx", dx, want, e + 8 * E32 * want.abs() + half_step(t) * want.abs() * (1 + 2.0 ** -8) + TINY[t])
+    within("db", db, dy.to(F64).sum(0), 8 * E32 * dy.to(F64).abs().sum(0) + half_step(t) * dy.to(F64).sum(0).abs() * 1.01 + TINY[t])
