@@ -86,3 +86,23 @@ def test_layer_norm_backward_of_large_constant_rows(gpu, c, t):
     e = rs * (4 * E32 * (h.abs() + mean.abs()) + (chain + 2) * E32 * h.abs().mean(1, keepdim=True))
     within("dx", dx, want, e + 8 * E32 * want.abs() + half_step(t) * want.abs() * (1 + 2.0 ** -8) + TINY[t])
     within("db", db, dy.to(F64).sum(0), 8 * E32 * dy.to(F64).abs().sum(0) + half_step(t) * dy.to(F64).sum(0).abs() * 1.01 + TINY[t])
+
+
+@pytest.mark.parametrize("t,last", [("f32", 200), ("bf16", 200), ("f16", 86)])
+def test_gelu_tail(gpu, t, last):
+    """gelu and its slope from z = -1/16 to -12.5 (f16: -5.4) keep the type's relative precision: Phi's formula is off
+    by 1.3e-5 relatively, exp(-z^2 / 2) by its argument's three roundings (3 x 78 x 2^-24 = 1.4e-5), together
+    at most 4e-5 with the products'; then one rounding, or two that are the same (dz and dx = dz 1)."""
+    from gwn_amd.layers import linear_act
+    z = (-torch.arange(1, last + 1) / 16).to(TYPES[t])[:, None]
+    w = torch.ones(1, 1, device=gpu, dtype=TYPES[t])
+    phi = torch.exp(-z.to(F64) ** 2 / 2) / (2 * torch.pi) ** 0.5
+    cdf = 0.5 * torch.special.erfc(-z.to(F64) / 2 ** 0.5)
+    value, slope = z.to(F64) * cdf, cdf + z.to(F64) * phi
+    u, off = half_step(t) * (1 + 2.0 ** -8), 4e-5
+    for rows in (slice(0, last), slice(last - 20, last)):  # of tiles, and of few rows
+        x = z[rows].to(gpu).requires_grad_()
+        y = linear_act(x, w, act="gelu")
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        within("y", y, value[rows], (u + off) * value[rows].abs() + TINY[t])
+        within("dx", dx, slope[rows], u * slope[rows].abs() + off * (cdf + z.to(F64).abs() * phi)[rows] + TINY[t])
