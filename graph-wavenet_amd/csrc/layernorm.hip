@@ -481,7 +481,7 @@ __global__ __launch_bounds__(THREADS) void ln_cols_long_kernel(const LnBwd p) {
   }
 }
 
-// out[k] = sum over parts of part[.][k]: 32 columns x 32 lanes of parts a workgroup, fixed order.  The
+// out[k] = sum over parts of part[.][k]: 32 columns x 32 lanes of parts a workgroup, in part_sum's order.  The
 // workgroups walk the columns: a grid has fewer than 2^32 threads, and columns go up to 2^31.
 constexpr long REDUCE_GRID = 1 << 16;
 template <typename W>
@@ -490,16 +490,10 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* part, int 
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   for (long first = (long)blockIdx.x * 32; first < 2L * c; first += (long)gridDim.x * 32) {
     const long k = first + tx;
-    float v = 0.0f;
-    if (k < 2L * c)
-#pragma unroll 8
-      for (int q = ty; q < nparts; q += 32) v += part[(long)q * 2 * c + k];
-    s[ty][tx] = v;
+    s[ty][tx] = k < 2L * c ? part_sum(part + k, 2L * c, ty, nparts) : 0.0f;
     __syncthreads();
     if (ty == 0 && k < 2L * c) {
-      v = 0.0f;
-#pragma unroll
-      for (int q = 0; q < 32; ++q) v += s[q][tx];
+      const float v = pair_sum<32, 33>(&s[0][tx]);
       if (k < c) {
         if (dgamma) dgamma[k] = (W)v;
       } else if (dbeta) {

@@ -774,24 +774,15 @@ __global__ __launch_bounds__(256) void dz_kernel(const Dz p) {
   }
 }
 
-// the stripes' sums, 32 columns x 32 lanes of stripes a workgroup (4 to 5 us), fixed order
+// the stripes' sums, 32 columns x 32 lanes of stripes a workgroup (4 to 5 us), in part_sum's order
 template <typename T>
 __global__ __launch_bounds__(1024) void colsum_kernel(const float* part, int nparts, int n, T* out) {
   __shared__ float s[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const long k = (long)blockIdx.x * 32 + tx;
-  float v = 0.0f;
-  if (k < n)
-#pragma unroll 8
-    for (int q = ty; q < nparts; q += 32) v += part[(long)q * n + k];
-  s[ty][tx] = v;
+  s[ty][tx] = k < n ? part_sum(part + k, n, ty, nparts) : 0.0f;
   __syncthreads();
-  if (ty == 0 && k < n) {
-    v = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 32; ++q) v += s[q][tx];
-    out[k] = (T)v;
-  }
+  if (ty == 0 && k < n) out[k] = (T)pair_sum<32, 33>(&s[0][tx]);
 }
 
 // ---- plans ------------------------------------------------------------------------------------------

@@ -106,3 +106,22 @@ def test_gelu_tail(gpu, t, last):
         dx, = torch.autograd.grad(y, x, torch.ones_like(y))
         within("y", y, value[rows], (u + off) * value[rows].abs() + TINY[t])
         within("dx", dx, slope[rows], u * slope[rows].abs() + off * (cdf + z.to(F64).abs() * phi)[rows] + TINY[t])
+
+
+def test_sums_of_many_rows_have_short_chains(gpu):
+    """The gradients of a bias and a norm's bias in fp32: one term is 1, the others so small that 31 of 32 equal sums
+    each fall under half a step of 1 if added to it one by one, which would lose 31 e.  A chain of n additions
+    loses n e at most: the norm's rows are added in chains of 6 (a group's rows), 3 (a wave's groups), 3 (waves),
+    7 and 5 (partial rows), the product's in chains of 4, 4, 7 and 5."""
+    from gwn_amd.layers import layer_norm, linear_act
+    for m, c, share, chain in ((172224, 32, 5440, 24), (16384, 512, 512, 20)):
+        dy = torch.full((m, c), 2.0 ** -24 * (1 - 2.0 ** -6) / share, device=gpu)
+        dy[0] = 1
+        b = torch.zeros(c, device=gpu, requires_grad=True)
+        if c == 32:
+            y = layer_norm(torch.randn(m, c, device=gpu), None, b)
+        else:
+            y = linear_act(torch.randn(m, 8, device=gpu), torch.zeros(c, 8, device=gpu), b)
+        db, = torch.autograd.grad(y, b, dy)
+        want = dy.double().sum(0).cpu()
+        within("db", db, want, (chain + 1) * E32 * want)
