@@ -299,16 +299,15 @@ __global__ __launch_bounds__(256) void wgrad_bf16_kernel(const WgB p) {
   const __amdgpu_buffer_rsrc_t rx = rsrc(p.X, (long)r1 * p.ldx * 4);
   const bool bias = kt == 0;
 
+  // Rows from r1 on: the first byte past the buffer, so zeros.  No branch: in one the loads wait for each other.
+  const unsigned ly = (unsigned)p.ldy * 4, lx = (unsigned)p.ldx * 4;
   float yv[16], xv[16];
   auto gload = [&](int rs) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int row = rs + 16 * rh + e;
-      const bool ok = row < r1;
-      yv[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                            ry, ok ? (int)(((long)row * p.ldy + j0 + scol) * 4) : OOR, 0, 0));
-      xv[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                            rx, ok ? (int)(((long)row * p.ldx + k0 + scol) * 4) : OOR, 0, 0));
+      const unsigned row = rs + 16 * rh + e < r1 ? rs + 16 * rh + e : r1;
+      yv[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(ry, row * ly + (j0 + scol) * 4, 0, 0));
+      xv[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rx, row * lx + (k0 + scol) * 4, 0, 0));
     }
   };
   float bsum = 0.0f;
@@ -346,7 +345,9 @@ __global__ __launch_bounds__(256) void wgrad_bf16_kernel(const WgB p) {
   __syncthreads();
   for (int st = 0; st < nst; ++st) {
     const int buf = st & 1;
-    if (st + 1 < nst) gload(r0 + (st + 1) * WBR);
+    // Past the last step too: zeros into the buffer that nobody reads.  Behind a branch the compiler moves the loads
+    // down to the conversions, or copies their registers, which waits for them.
+    gload(r0 + (st + 1) * WBR);
 #pragma unroll
     for (int ks = 0; ks < WBR / 16; ++ks) {
       bf16x8n af[2], bf[2];
@@ -359,7 +360,8 @@ __global__ __launch_bounds__(256) void wgrad_bf16_kernel(const WgB p) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf[t], acc[i][t], 0, 0, 0);
     }
-    if (st + 1 < nst) swrite(buf ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    swrite(buf ^ 1);
     __syncthreads();
   }
   float* out = p.part + (long)c * ((long)p.J * p.Kc + p.J);
