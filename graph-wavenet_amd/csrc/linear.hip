@@ -180,14 +180,18 @@ __device__ __forceinline__ u32x4 rsrc(const void* base, unsigned bytes) {
 // 16 bytes a lane from `off` of the resource to LDS at `lds` + 16 lane.  In assembly because the
 // compiler waits for every such load before the next transposed LDS read, whichever buffer either
 // touches; nothing is written to registers, and the loop below waits for vmcnt itself.
+// m0 needs one state before the load; five pass after the assembly begins, since the compiler does not look into it
+// for the five that a vector instruction's scalar result (a reloaded spill) needs before a load takes it.
+// m0 is reserved, and the compiler refuses it as a clobber: it sets it before each use of its own, and has
+// none in this kernel.
 __device__ __forceinline__ void load_lds(u32x4 rs, unsigned off, unsigned lds) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
+      "s_nop 3\n\t"
       "buffer_load_dwordx4 %1, %2, 0 offen lds"
       :
       : "s"(lds), "v"(off), "s"(rs)
-      : "memory");  // m0 is reserved: the compiler sets it before each use of its own, and has none here
+      : "memory");
 }
 
 // where in a K row piece 0 lies: the 16 rows that one LDS cycle reads together (256 bytes; lanes 0-3,

@@ -50,3 +50,13 @@ def test_tile_loads_to_lds_have_m0_to_themselves(kernels):
                 if re.search(r"\bm0\b", a):
                     assert a.startswith("s_mov_b32 m0,") and b.startswith("s_nop") and c.endswith("offen lds"), (k, a)
     assert n >= 60
+
+
+def test_tile_loads_wait_for_scalar_results(kernels):
+    """Five states pass in these loads' assembly, which the compiler's hazard handling does not look into, before
+    they take scalar registers that a vector instruction may have written right before."""
+    for k, code in kernels.items():
+        if "gemm_kernel" in k:
+            for a, b in zip(code, code[1:]):
+                if b.endswith("offen lds"):
+                    assert a.startswith("s_nop") and int(a.split()[1], 0) >= 3, (k, a)
