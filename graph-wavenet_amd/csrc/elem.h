@@ -54,7 +54,7 @@ __device__ __forceinline__ Pack<T, N> load_odd(const T* p) {
 // ceil(p 2^24).  The 64-bit key is two rounds of the SplitMix64 finaliser (Steele, Lea and Flood
 // 2014) over seed, salt and the high half of i; its low word starts the 32-bit mix of the low half
 // (the constants of gwn_mix32), its high word enters between that mix's two multiplies, so that two
-// keys' streams are not shifts of one another.  Two multiplies per element, no memory: the mask is
+// keys' streams are not shifts of one another.  Three multiplies per element, no memory: the mask is
 // the same in every kernel that applies or differentiates it.
 struct Drop {
   const unsigned long long* seed_ptr;

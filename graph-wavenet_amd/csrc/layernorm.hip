@@ -14,9 +14,12 @@
 // and a second launch adds the partial rows in a fixed order.  Rows longer than a workgroup's
 // registers are looped over (they stay in the L2 cache between the passes).
 //
-// Measured, 20800 x 4096 in bf16: forward 67-71 us, backward 98 us + 5 us for the partial rows, 5.0 and 5.2
-// TB/s, as a large copy; 32 to 8192 channels run at 4.6 to 5.2 TB/s, odd widths at 2.5 to 5 (half-empty
-// waves, unaligned pieces), looped rows at 1.8 to 2.6.  Several vectors a lane took the backward's
+// Measured, 20800 x 4096 in bf16: forward 67-71 us, backward 98 us + 4 us for the partial rows, 5.0 and 5.2
+// TB/s, as a large copy.  Over widths (170 MB of x, forward and backward): rows of 32 to 8192 channels that fill their waves
+// with whole vectors run at 4.5 to 5.3 TB/s; others of these widths at 2.9 to 5.1 (idle lanes, unaligned pieces), and 16-bit
+// rows up to 16384 at 3.5 to 4.4.  Short rows in 16 bits leave lanes of the smallest group idle: 0.8 / 1.6 TB/s at 5
+// channels, 1.9 / 3.0 at 8, 2.4 / 2.2 at 12 (f32 2.8 to 5.0).  Looped rows (f32 from 8193 channels, 16 bits from 16385) take 1.8 to 3.2.
+// Several vectors a lane took the backward's
 // registers and with them the waves that hide its latency: 195 us with two.
 #include "elem.h"
 

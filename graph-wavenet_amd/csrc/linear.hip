@@ -147,9 +147,9 @@ template <int I> struct Int { static constexpr int value = I; };
 // address (swizzle, swizzle_m).  M rows of 16-bit values are read by ds_read_b64_tr_b16, which hands each
 // lane four k of its own column.  What lies outside
 // the matrices is a load past its buffer resource, which gives zeros.
-// Measured (bf16, one launch): 8192^3 842 us = 1306 TFLOP/s (a library product of the same operands
-// 1540), matrix units busy 72-77% of the cycles at the clock that the power limit leaves; 20800 x 2048 x
-// 8192 with gelu and z 737 us = 947 TFLOP/s.  With the loads in one burst behind the barrier and K rows
+// Measured (bf16, one launch): 8192^3 842-863 us = 1270-1306 TFLOP/s (a library product of the same operands
+// 1510-1560), matrix units busy 71-73% of the cycles (the library's 93%); 20800 x 2048 -> 8192 612-630 us, the units
+// busy 65% (the library 535-640 us, 74%), with gelu and z 727-737 us = 947 TFLOP/s.  With the loads in one burst behind the barrier and K rows
 // swizzled by row & 7 (half of the LDS cycles conflicts) 8192^3 took 899 us; 64 bytes of k in 4 or 5
 // buffers 920, 128 x 256 tiles two a compute unit 1069, 4 waves of 128 x 128 810 but 10% more with an
 // epilogue; fragment reads between the products, and wave priorities, changed nothing.
@@ -554,7 +554,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
 // v_mfma_f32_16x16x32 (16-bit) or 16x16x4 fragments.  A workgroup has 16 columns (w rows), its waves
 // split the contraction: 4 loads of 16 bytes a lane, 256 bytes of each w row, are in flight a wave and
 // turn, x's pieces come from the caches.  The waves' sums meet in LDS, then the epilogue.  Rows may
-// start anywhere and have any length.
+// start anywhere and have any length.  1 x 1024 -> 4096: bf16 and f16 4.0 us, f32 6.4 (w read at 2.1 and 2.6 TB/s);
+// 16 x 4096 -> 4096 11.7 and 19.5 us (2.9 and 3.5 TB/s); 12 x 1999 -> 1030 7.5 to 8.8 us in all three.
 struct Few {
   const void* x; long ldx;
   const void* w; long ldw;

@@ -759,7 +759,8 @@ int gwn_window_batch(const double* series, const double* tod, const double* dow,
  * extend linear (model.py:24-30), the BatchNorm (model.py:152, 236) and the dropout (model.py:54)
  * of the graph convolution; the reference has no counterpart.  Sums, statistics and gradients'
  * partial sums are fp32 whatever the element type, every output is rounded once, and reductions
- * have a fixed order.  Pointers are aligned to their element, no more; a leading dimension counts
+ * have a fixed order; activations of 16-bit elements are evaluated to within 4e-5 of their terms.
+ * Pointers are aligned to their element, no more; a leading dimension counts
  * elements and is at least the row's length.  Outputs must not overlap inputs unless said.
  * ------------------------------------------------------------------------------------------- */
 typedef enum gwn_elem { GWN_ELEM_F32 = 0, GWN_ELEM_F16 = 1, GWN_ELEM_BF16 = 2 } gwn_elem;
@@ -782,7 +783,7 @@ typedef enum gwn_act {
 int gwn_dropout(const void* x, const void* residual, void* y, long count, int elem,
                 const unsigned long long* seed_ptr, unsigned long long salt, double drop_p, hipStream_t stream);
 
-/* Layer norm over the c values of each of `rows` rows:
+/* Layer norm over the c values (at most 2^30) of each of `rows` rows:
  *   mean = sum x / c, rstd = 1/sqrt(sum (x - mean)^2 / c + eps), y = (x - mean) rstd gamma + beta.
  * gamma / beta [c] (NULL = 1 / 0) are of type `elem`, or f32 with params_f32 != 0.  mean / rstd
  * [rows] f32 (both or neither NULL) are kept for the backward.  y may be x (same ld). */
@@ -800,7 +801,7 @@ long gwn_layernorm_bwd_workspace_floats(long rows, int c, int elem);
  * NULL, residual [M][ld_res] or NULL, y [M][ldy]; D is gwn_dropout's mask on element m N + n (drop_p
  * 0 = none, seed_ptr unused).  z [M][ldz] (NULL = no backward follows, or act NONE): the pre-activation
  * for the backward, float for f32 elements and otherwise f16 (past its range an infinity; with relu a
- * positive value stays one).  y may be residual (same ld). */
+ * positive value stays one).  y may be residual (same ld).  M is at most 2^30, N and K 2^20. */
 typedef struct gwn_linear_args {
   const void* x; long ldx;
   const void* w; long ldw;
