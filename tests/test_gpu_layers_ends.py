@@ -4,7 +4,7 @@ values near the types' ends, an activation's tail, long sums.  Oracles and bound
 import pytest
 import torch
 
-from test_gpu_layers import E32, F64, LinearCase, TINY, TYPES, half_step, mask, within
+from test_gpu_layers import E32, F64, LinearCase, TINY, TYPES, half_step, mask, run_linear, within
 
 pytestmark = pytest.mark.gpu
 
@@ -40,11 +40,46 @@ def test_linear_act_most_rows(gpu):
     assert not dx.any()
 
 
-def test_layer_norm_many_channels(gpu):
-    """A row of more than 2^26 channels: its parameters' gradients are one term each.  Its values are +-1 in turn, so
-    its statistics are exact but for 8 roundings of fp32."""
+def test_linear_act_row_limit(gpu):
+    """2^30 rows, the most, of one channel: values at the ends; the weight's and the bias's gradients are sums of 2^30
+    products, zeros but for 64 of them."""
+    from gwn_amd.layers import linear_act
+    m, n = 2 ** 30, 32
+    x = torch.zeros(m, 1, device=gpu, dtype=torch.float16)
+    at = torch.cat([torch.arange(n), torch.arange(m - n, m)]).to(gpu)
+    g = torch.Generator().manual_seed(4)
+    xs = torch.randint(-8, 9, (2 * n, 1), generator=g).double() / 4
+    ds = torch.randint(-8, 9, (2 * n, 1), generator=g).double() / 8
+    x[at] = xs.to(gpu).half()
+    w = torch.full((1, 1), 1.5, device=gpu, dtype=torch.float16)
+    b = torch.full((1,), 0.25, device=gpu, dtype=torch.float16)
+    for v in (x, w, b):
+        v.requires_grad_()
+    y = linear_act(x, w, b, act="relu")
+    z = xs * 1.5 + 0.25  # exact, as all that follows: small multiples of 1/64
+    assert torch.equal(y[at].double().cpu(), z.clamp(min=0)) and bool((y[n:m - n] == 0.25).all())
+    dy = torch.zeros_like(y)
+    dy[at] = ds.to(gpu).half()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    dz = ds * (z > 0)
+    assert torch.equal(dx[at].double().cpu(), dz * 1.5) and not dx[n:m - n].any()
+    assert dw.item() == float((dz * xs).sum()) and db.item() == float(dz.sum())
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("m,k,n", [(3, 2 ** 20, 40), (40, 2 ** 20 - 1, 3), (3, 40, 2 ** 20), (33, 9, 2 ** 20 - 7)])
+def test_linear_act_most_channels(gpu, t, m, k, n):
+    c = LinearCase(m, k, n, t, "silu", True, True, 0.3)
+    y, got = run_linear(c, gpu)
+    c.check(y=y, **got)
+
+
+@pytest.mark.parametrize("c", [2 ** 26 + 40, 2 ** 30])
+def test_layer_norm_many_channels(gpu, c):
+    """A row of more than 2^26 channels, up to the most: its parameters' gradients are one term each.  Its values are
+    +-1 in turn, so its statistics are exact but for 8 roundings of fp32."""
     from gwn_amd.layers import layer_norm
-    c, t = 2 ** 26 + 40, torch.bfloat16
+    t = torch.bfloat16
     x = torch.ones(1, c, device=gpu, dtype=t)
     x[:, 1::2] = -1
     w, b = torch.ones(c, device=gpu, dtype=t), torch.full((c,), 0.25, device=gpu, dtype=t)
