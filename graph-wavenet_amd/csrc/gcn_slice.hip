@@ -1122,10 +1122,7 @@ void ensure_lds_attr(K kern) {
 int bn_part_tail(float* bn_part, int slices, int c, hipStream_t s) {
   const long slots = gwn_bn_part_slots(slices);
   if (!bn_part || slots <= slices) return GWN_OK;
-  return hipMemsetAsync(bn_part + (long)slices * 3 * c, 0, (size_t)(slots - slices) * 3 * c * sizeof(float), s) ==
-                 hipSuccess
-             ? GWN_OK
-             : gwn_set_error(GWN_ERR_HIP, "gcn_fwd: BN partial tail memset failed");
+  return gwn_zero_floats(bn_part + (long)slices * 3 * c, (slots - slices) * 3 * c, s);
 }
 
 }  // namespace

@@ -27,6 +27,9 @@ int gwn_debug_range(const void* p, long bytes, const char* what);
 
 int gwn_set_error(int code, const char* msg);
 
+// p[0 .. n) = 0 by a kernel: a memset that a captured graph records has left wrong values on later replays
+int gwn_zero_floats(float* p, long n, hipStream_t s);
+
 // ---------------------------------------------------------------------------------------------
 // Generic fp32 MFMA GEMM (gemm.hip).  C(m,n) = epi(alpha * sum_k A(m,k) B(k,n)).
 //

@@ -958,6 +958,10 @@ int grid_for(long total, int block = 256) {
   return (int)g;
 }
 
+__global__ __launch_bounds__(256) void zero_floats_kernel(float* p, long n) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.0f;
+}
+
 }  // namespace
 
 // =============================================================================================
@@ -980,6 +984,14 @@ int gwn_launch_status(const char* file, int line) {
   char buf[256];
   snprintf(buf, sizeof(buf), "%s (%s:%d)", hipGetErrorString(e_), file, line);
   return gwn_set_error(GWN_ERR_HIP, buf);
+}
+
+int gwn_zero_floats(float* p, long n, hipStream_t s) {
+  if (n <= 0) return GWN_OK;
+  const long want = (n + 255) / 256;
+  zero_floats_kernel<<<(int)(want < 2048 ? want : 2048), 256, 0, s>>>(p, n);
+  GWN_CHECK_LAUNCH();
+  return GWN_OK;
 }
 
 // debugging (GWN_SYNC_CHECK): does [p, p + bytes) lie inside one device allocation?
@@ -1270,10 +1282,7 @@ int gwn_gated_tcn_bwd(const gwn_tcn_bwd_args* a, hipStream_t s) {
     GWN_CHECK_LAUNCH();
     return GWN_OK;
   }
-  if (a->accumulate_dx && a->acc_row0 > 0) {
-    if (hipMemsetAsync(a->dx, 0, (size_t)a->acc_row0 * c * sizeof(float), s) != hipSuccess)
-      return gwn_set_error(GWN_ERR_HIP, "gated_tcn_bwd: memset failed");
-  }
+  if (a->accumulate_dx && a->acc_row0 > 0 && (rc = gwn_zero_floats(a->dx, (long)a->acc_row0 * c, s))) return rc;
   d = gemm_zero();
   d.A = a->dfg; d.lda_m = 2 * co; d.lda_k = 1; d.a_kin = 2 * co; d.a_row_shift = -a->dilation * P;
   d.a_rows = (int)rows;
@@ -1363,10 +1372,8 @@ static int gcn_fwd_unfolded(const gwn_gcn_args* a, hipStream_t s) {
   bn_partial_kernel<<<slices, 256, 0, s>>>(a->z, a->rows, co, a->bn_partials);  // one chunk per slice
   GWN_CHECK_LAUNCH();
   const long slots = gwn_bn_part_slots(slices);  // the slots past the slices hold no rows
-  if (slots > slices && hipMemsetAsync(a->bn_partials + (long)slices * 3 * co, 0,
-                                       (size_t)(slots - slices) * 3 * co * sizeof(float), s) != hipSuccess)
-    return gwn_set_error(GWN_ERR_HIP, "gcn_fwd: BN partial tail memset failed");
-  return GWN_OK;
+  if (slots <= slices) return GWN_OK;
+  return gwn_zero_floats(a->bn_partials + (long)slices * 3 * co, (slots - slices) * 3 * co, s);
 }
 
 static int gcn_w_ksplit(int rows, int c, int width) { return pick_ksplit(c, width, rows); }

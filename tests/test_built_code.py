@@ -60,3 +60,12 @@ def test_tile_loads_wait_for_scalar_results(kernels):
             for a, b in zip(code, code[1:]):
                 if b.endswith("offen lds"):
                     assert a.startswith("s_nop") and int(a.split()[1], 0) >= 3, (k, a)
+
+
+def test_no_memsets():
+    """Memory is cleared by kernels: a memset that a captured graph records has left wrong values on later replays,
+    and every entry may be captured."""
+    from gwn_amd import _lib
+    names = subprocess.run(["nm", "-D", "--undefined-only", _lib.LIB_PATH], check=True, stdout=subprocess.PIPE,
+                           text=True).stdout
+    assert "hipLaunchKernel" in names and "hipMemset" not in names
