@@ -4,7 +4,7 @@ values near the types' ends, an activation's tail, long sums.  Oracles and bound
 import pytest
 import torch
 
-from test_gpu_layers import E32, F64, LinearCase, TINY, TYPES, half_step, mask, run_linear, within
+from test_gpu_layers import E32, F64, LinearCase, TINY, TYPES, act64, half_step, mask, run_linear, within
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,22 @@ def test_sums_of_many_rows_have_short_chains(gpu):
         db, = torch.autograd.grad(y, b, dy)
         want = dy.double().sum(0).cpu()
         within("db", db, want, (chain + 1) * E32 * want)
+
+
+@pytest.mark.parametrize("t,last", [("f32", 200), ("bf16", 200), ("f16", 86)])
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
+def test_sigmoid_tails(gpu, act, t, last):
+    """The same for the activations z s(u), s = 1 / (1 + exp(-u)): exp is off by its argument's roundings, u's among
+    them (4 x |u| 2^-24, and |u| is at most 88 where the value is above fp32's smallest), together under
+    4e-5 of each term of the slope s + z s (1 - s) u'; an s under fp32's smallest normal number may be 0."""
+    from gwn_amd.layers import linear_act
+    z = (-torch.arange(1, last + 1) / 16).to(TYPES[t])[:, None]
+    w = torch.ones(1, 1, device=gpu, dtype=TYPES[t])
+    value, slope = act64(z.to(F64), act)
+    s = value / z.to(F64)
+    u, off = half_step(t) * (1 + 2.0 ** -8), 4e-5
+    x = z.to(gpu).requires_grad_()
+    y = linear_act(x, w, act=act)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    within("y", y, value, (u + off) * value.abs() + z.to(F64).abs() * 2.0 ** -126 + TINY[t])
+    within("dx", dx, slope, u * slope.abs() + off * (s.abs() + (slope - s).abs()) + (1 + (slope / s).abs()) * 2.0 ** -126 + TINY[t])
